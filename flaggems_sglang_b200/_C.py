@@ -75,6 +75,18 @@ class FusedArgs(_SizedStructure):
     ]
 
 
+class Fp8Args(_SizedStructure):
+    """Mirror of struct fmoe_fp8_args."""
+
+    _fields_ = [
+        ("struct_size", c_uint32), ("x_dtype", c_int32), ("activation", c_int32), ("reserved", c_int32),
+        ("T", c_int64), ("K", c_int64), ("N", c_int64), ("I", c_int64),
+        ("x", c_void_p), ("x_scale", c_void_p), ("w", c_void_p), ("w_scale", c_void_p), ("w2", c_void_p),
+        ("w2_scale", c_void_p), ("bias", c_void_p), ("addend", c_void_p), ("out", c_void_p), ("out_scale", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 class RouteArgs(Structure):
     """Mirror of struct fmoe_route_args."""
 
@@ -115,6 +127,14 @@ SIGNATURES = {
     "fmoe_fused_moe": (c_int, [POINTER(FusedArgs), POINTER(RouteArgs), c_void_p]),
     "fmoe_fused_experts_sorted_workspace_bytes": (c_int64, [POINTER(FusedArgs)]),
     "fmoe_fused_experts_sorted": (c_int, [POINTER(FusedArgs), c_void_p, c_void_p, c_void_p, c_void_p]),
+    "fmoe_fp8_linear_workspace_bytes": (c_int64, [POINTER(Fp8Args)]),
+    "fmoe_fp8_linear": (c_int, [POINTER(Fp8Args), c_void_p]),
+    "fmoe_fp8_gate_up_workspace_bytes": (c_int64, [POINTER(Fp8Args)]),
+    "fmoe_fp8_gate_up": (c_int, [POINTER(Fp8Args), c_void_p]),
+    "fmoe_fp8_mlp_workspace_bytes": (c_int64, [POINTER(Fp8Args)]),
+    "fmoe_fp8_mlp": (c_int, [POINTER(Fp8Args), c_void_p]),
+    "fmoe_rms_norm_quant": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float,
+                                    c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "fmoe_static_scratch_bytes": (c_int64, []),
     "fmoe_fused_experts_static": (c_int, [POINTER(FusedArgs), c_void_p]),
     "fmoe_ep_buffer_create": (c_int, [c_int64, POINTER(c_void_p), c_void_p]),

@@ -9,7 +9,7 @@
 namespace fmoe {
 namespace {
 
-enum class RowMode { kMap, kScatter, kInPlace, kExpert };
+enum class RowMode { kMap, kScatter, kInPlace, kExpert, kTokens };  // kTokens: row p to row p, late trigger
 
 // Source row of output position p: p itself without a map; with a map, the map's entry divided by map_div,
 // or p when map_div is 0 (the map then only marks padding).  -1 = padding position.
@@ -70,7 +70,8 @@ quant_group128_kernel(const InT* __restrict__ x, int64_t rows_out, int64_t K, co
       for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
       if (p < limit) {
         const int64_t r = MODE == RowMode::kExpert ? (int64_t)blockIdx.y * map_div + p
-                          : (MODE == RowMode::kInPlace ? pos[p] : mapped_row(row_map, map_div, sentinel, p));
+                          : (MODE == RowMode::kInPlace ? pos[p]
+                             : (MODE == RowMode::kTokens ? p : mapped_row(row_map, map_div, sentinel, p)));
         if constexpr (MODE == RowMode::kExpert) pu[u] = base + p;
         if constexpr (MODE == RowMode::kInPlace) pu[u] = r;
         real[u] = r >= 0;
@@ -475,6 +476,15 @@ int fmoe::run_quant_rows(const void* x, int64_t numel, int64_t K, const int32_t*
   else if (K <= 4096) go(quant_row_kernel<32, 16, RowMode::kInPlace>, ceil_div<int64_t>(numel, 8));
   else go(quant_row_kernel<256, 8, RowMode::kInPlace>, numel);
   return launch_status("quant_rows");
+}
+
+int fmoe::run_quant_tokens(const void* x, int64_t T, int64_t K, void* q, float* scale, cudaStream_t st) {
+  FMOE_REQUIRE(K > 0 && K % 128 == 0, "quant_tokens: bad K %lld", (long long)K);
+  FMOE_REQUIRE(x && q && scale && aligned16(x) && aligned16(q), "quant_tokens: null or misaligned pointer");
+  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div<int64_t>(T * (K / 128), 64), 148 * 8));
+  launch_pdl(quant_group128_kernel<__nv_bfloat16, RowMode::kTokens>, dim3(grid), dim3(256), 0, st, (const __nv_bfloat16*)x, T, K, nullptr, 1,
+             0, nullptr, (uint8_t*)q, scale, nullptr);
+  return launch_status("quant_tokens");
 }
 
 int fmoe::run_quant_slots(const float* x, int64_t numel, int64_t K, const int32_t* slot_pos, void* q, float* scale, cudaStream_t st) {

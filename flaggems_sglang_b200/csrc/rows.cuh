@@ -20,6 +20,9 @@ int run_quant_slots(const float* x, int64_t numel, int64_t K, const int32_t* slo
 int run_quant_experts(const float* x, int64_t numel, int64_t K, int num_experts, const int32_t* table, int max_rows, void* q,
                       float* scale, cudaStream_t st);
 
+// bf16 rows -> e4m3 with a scale per 128 channels; the next kernel starts only after this one's own wait
+int run_quant_tokens(const void* x, int64_t T, int64_t K, void* q, float* scale, cudaStream_t st);
+
 #if defined(__CUDACC__)
 // Scale of a group of 128 channels with this largest magnitude.
 __device__ __forceinline__ float group_scale(float amax) { return __fdiv_rn(fmaxf(amax, 1e-10f), 448.0f); }
@@ -45,6 +48,21 @@ __device__ __forceinline__ uint2 quant8(const float (&v)[8], float s, float r, b
     }
   }
   return make_uint2(lo, hi);
+}
+
+// Four values likewise.
+__device__ __forceinline__ uint32_t quant4(const float (&v)[4], float s, float r, bool finite) {
+  uint32_t w = 0;
+  if (finite) {
+    auto pair = [](float a, float b) {
+      return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    };
+    w = pair(div_by_shared(v[0], s, r), div_by_shared(v[1], s, r)) | (pair(div_by_shared(v[2], s, r), div_by_shared(v[3], s, r)) << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (uint32_t)f32_to_e4m3_bits(__fdiv_rn(v[i], s)) << (8 * i);
+  }
+  return w;
 }
 #endif
 

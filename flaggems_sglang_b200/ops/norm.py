@@ -1,0 +1,58 @@
+"""Residual addition, root-mean-square norm and e4m3 quantisation in one kernel (csrc/norm.cu)."""
+from __future__ import annotations
+
+import torch
+
+from .. import _C
+
+
+def _rows(t: torch.Tensor) -> bool:
+    """Rows that the kernel reads in place: contiguous channels, rows at multiples of 16 bytes that do not overlap."""
+    per16 = 16 // t.element_size()
+    return (t.stride(1) == 1 and (t.shape[0] == 1 or (t.stride(0) >= t.shape[1] and t.stride(0) % per16 == 0))
+            and t.data_ptr() % 16 == 0)
+
+
+def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+                       per_token: bool = False, return_norm: bool = False):
+    """x [rows, K] (bf16 or fp32) -> (q e4m3 [rows, K], scale f32 [rows, K/128]); the input of the e4m3 layers.
+
+    With ``residual [rows, K]`` (x's type) the norm is of ``x + residual``, and ``residual`` holds that sum, rounded to its type,
+    afterwards (in place).  ``y = h / sqrt(mean(h^2) + eps) * weight`` is computed in fp32 and rounded once, by the rule of
+    `per_token_group_quant_fp8`; with ``per_token`` by that of `per_token_quant_fp8` (scale [rows]).  ``return_norm`` appends
+    y in x's type, for what reads the layer's input unquantised (a router, bf16 experts).
+    K is a multiple of 128 (``per_token``: of 8), at most 16384.  Rows of x and residual may be strided; weight is bf16 or fp32 [K].
+    """
+    dev = _C.require_cuda(x, weight, residual)
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("x must be a 2-D bf16 or fp32 tensor")
+    rows, K = x.shape
+    if weight.shape != (K,) or weight.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("weight must be a bf16 or fp32 tensor of x's row length")
+    if K == 0 or K > 16384 or K % (8 if per_token else 128):
+        raise ValueError(f"rows of {K} channels: a multiple of {8 if per_token else 128} up to 16384 is needed")
+    if not _rows(x):
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    weight = weight.contiguous()
+    if weight.data_ptr() % 16:
+        weight = weight.clone()
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError("residual must have x's shape and type")
+        if not _rows(residual):
+            raise ValueError("residual is updated in place: its channels must be contiguous and its rows start at multiples of 16 bytes")
+    q = torch.empty(rows, K, dtype=torch.float8_e4m3fn, device=dev)
+    s = torch.empty((rows,) if per_token else (rows, K // 128), dtype=torch.float32, device=dev)
+    norm = torch.empty(rows, K, dtype=x.dtype, device=dev) if return_norm else None
+    with _C.on_device(dev):
+        _C.check(_C.lib().fmoe_rms_norm_quant(
+            x.data_ptr(), x.stride(0) if rows > 1 else K, _C.ptr(residual),
+            (residual.stride(0) if rows > 1 else K) if residual is not None else K,
+            _C.DTYPE_CODE[x.dtype], weight.data_ptr(), _C.DTYPE_CODE[weight.dtype], rows, K, eps, int(per_token), q.data_ptr(),
+            s.data_ptr(), _C.ptr(norm), _C.stream_ptr(dev)))
+    return (q, s, norm) if return_norm else (q, s)
+
+
+__all__ = ["rms_norm_quant_fp8"]

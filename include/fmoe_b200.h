@@ -331,6 +331,59 @@ int fmoe_fused_experts_sorted(const fmoe_fused_args* args, const int32_t* topk_i
                               const float* gate_scal, void* stream);
 
 /*
+ * Dense products of e4m3 operands with block scales: what a layer of this format computes beside its routed experts.  No
+ * counterpart in the reference, which rejects fp8 (src/flaggems_sglang/ops/fused_moe.py:170-185).
+ *   x [T, K] bf16 (quantised in the call by the rule of fmoe_quant_fp8_group128) or e4m3 with x_scale [T, K/128] f32
+ *   w [rows, K] e4m3 with w_scale [ceil(rows/128), K/128] f32, one scale per 128 x 128 block (the last one of ragged rows holds fewer)
+ *   K (and I) multiples of 128; partial sums are f32, the result is rounded once.
+ * fmoe_fp8_linear : w has N rows (N a multiple of 8); out [T, N] bf16 = x w^T (+ bias [N] f32) (+ addend [T, N] bf16)
+ * fmoe_fp8_gate_up: w has 2I rows (gate rows, then up rows; I a multiple of 128); h = act(x w_gate^T) * (x w_up^T) in f32, quantised
+ *                   by the same rule: out [T, I] e4m3, out_scale [T, I/128] f32
+ * fmoe_fp8_mlp    : both: h as above (it stays in the workspace), out [T, N] bf16 = h w2^T (+ bias) (+ addend); w2 [N, I] e4m3 with
+ *                   w2_scale [ceil(N/128), I/128].  The shared expert of a layer, whose `addend` is the routed experts' result.
+ * out may be addend itself, and otherwise overlaps no input.  The workspace (256-byte aligned) is used by one call at a time.
+ */
+typedef struct fmoe_fp8_args {
+  uint32_t struct_size;  /* sizeof(fmoe_fp8_args) as the caller compiled it */
+  int32_t x_dtype;       /* FMOE_BF16 | FMOE_E4M3 */
+  int32_t activation;    /* gate_up, mlp: FMOE_ACT_SILU | FMOE_ACT_GELU */
+  int32_t reserved;      /* 0 */
+  int64_t T, K, N, I;
+  const void* x;
+  const float* x_scale;
+  const void* w;
+  const float* w_scale;
+  const void* w2;
+  const float* w2_scale;
+  const float* bias;     /* optional */
+  const void* addend;    /* optional */
+  void* out;
+  float* out_scale;      /* gate_up */
+  void* workspace;       /* fmoe_fp8_*_workspace_bytes; may be NULL where that is 0 */
+  int64_t workspace_bytes;
+} fmoe_fp8_args;
+int64_t fmoe_fp8_linear_workspace_bytes(const fmoe_fp8_args* args);  /* pointers are not read; < 0 on error */
+int fmoe_fp8_linear(const fmoe_fp8_args* args, void* stream);
+int64_t fmoe_fp8_gate_up_workspace_bytes(const fmoe_fp8_args* args);
+int fmoe_fp8_gate_up(const fmoe_fp8_args* args, void* stream);
+int64_t fmoe_fp8_mlp_workspace_bytes(const fmoe_fp8_args* args);
+int fmoe_fp8_mlp(const fmoe_fp8_args* args, void* stream);
+
+/*
+ * Residual addition, root-mean-square norm and quantisation to e4m3 in one pass (no counterpart in the reference):
+ *   h = x + residual, rounded to their type and stored in `residual` (NULL: h = x)
+ *   y = h / sqrt(mean(h^2) + eps) * weight, in f32
+ *   q, scale: y by the rule of fmoe_quant_fp8_group128 (scale [rows, K/128]), or with per_token of fmoe_quant_fp8_per_token
+ *   (scale [rows]); norm (optional) [rows, K]: y rounded to x's type
+ * x, residual and norm are of `dtype` (FMOE_BF16 | FMOE_F32), weight [K] of weight_dtype (either).  x_stride and residual_stride are
+ * elements from row to row (>= K; rows start at multiples of 16 bytes); q and norm are dense.  K a multiple of 128 (per_token: of 8),
+ * at most 16384.  x may be residual itself; no other overlap of outputs and inputs.
+ */
+int fmoe_rms_norm_quant(const void* x, int64_t x_stride, void* residual, int64_t residual_stride, int dtype, const void* weight,
+                        int weight_dtype, int64_t rows, int64_t K, float eps, int per_token, void* q, float* scale, void* norm,
+                        void* stream);
+
+/*
  * fmoe_fused_experts for callers that cannot allocate device memory.  It has no counterpart in the
  * reference, which allocates its intermediates with torch on every call.
  *

@@ -1,0 +1,293 @@
+"""Dense e4m3 products with block scales (fp8_block_linear, fp8_gated_mlp) against their definition in 64 bits.
+
+Tolerances.  The products of e4m3 values are exact in fp32.  A sum of K of them, times two scales per block of 128, has an error of
+at most  (128 * 2^-23 + (K/128 + 16) * 2^-24) * sum |terms|:  128 additions inside a block, each off by at most one unit of a 24-bit
+significand whether the tensor core rounds or truncates, one fp32 addition per block, and at most 16 for the join of the cluster, the
+product of the scales, bias and addend.  The rounding to bf16 adds 2^-8 of the value.
+"""
+import ctypes
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+GROUP = 128
+
+
+def fg():
+    import flaggems_sglang_b200 as m
+
+    return m
+
+
+def status():
+    from flaggems_sglang_b200 import _C
+
+    _C.check_device_status()
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def rows(T, K, seed, wide=True):
+    x = torch.randn(T, K, generator=gen(seed), device="cuda")
+    if wide:  # groups of very different magnitude
+        x *= 10.0 ** torch.randint(-3, 3, (T, K // GROUP, 1), generator=gen(seed + 1), device="cuda").expand(-1, -1, GROUP).reshape(T, K)
+    return x
+
+
+def quant(x):
+    """Rows -> e4m3 and scales, by the quantiser's rule, in torch."""
+    v = x.float().view(x.shape[0], -1, GROUP)
+    s = v.abs().amax(-1).clamp_min(1e-10)
+    s = s / torch.full_like(s, 448.0)
+    return (v / s[..., None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(x.shape), s
+
+
+def weight(N, K, seed):
+    nb = -(-N // GROUP)
+    w = torch.zeros(nb * GROUP, K, device="cuda")
+    w[:N] = torch.randn(N, K, generator=gen(seed), device="cuda") / K ** 0.5
+    b = w.view(nb, GROUP, K // GROUP, GROUP)
+    b *= 10.0 ** torch.randint(-2, 2, (nb, 1, K // GROUP, 1), generator=gen(seed + 1), device="cuda")
+    s = b.abs().amax((1, 3)) / 448.0
+    return (b / s[:, None, :, None]).clamp(-448, 448).reshape(nb * GROUP, K)[:N].to(torch.float8_e4m3fn).contiguous(), s.contiguous()
+
+
+def values(q, s):
+    return q.double() * s.double().repeat_interleave(GROUP, 1)
+
+
+def weight_values(q, s):
+    return q.double() * s.double().repeat_interleave(GROUP, 0)[: q.shape[0]].repeat_interleave(GROUP, 1)
+
+
+def sum_error(K):
+    return 128 * 2.0 ** -23 + (K / 128 + 16) * 2.0 ** -24
+
+
+def check(out, xv, wv, more=None):
+    """out against xv wv^T + more, all in 64 bits."""
+    y, size = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    if more is not None:
+        y, size = y + more.double(), size + more.double().abs()
+    off = (out.double() - y).abs()
+    allowed = y.abs() * 2.0 ** -8 + size * sum_error(xv.shape[1]) * (1 + 2.0 ** -8)
+    assert torch.isfinite(out).all()
+    assert (off <= allowed).all(), f"off by {float((off - allowed).max())} more than allowed at {(off > allowed).nonzero()[:4].tolist()}"
+
+
+SHAPES = [
+    # T, K, N: single token, one block, ragged widths; every token tile; K that does and does not divide among the CTAs of a tile
+    (1, 128, 8), (1, 128, 128), (1, 7168, 2048), (2, 256, 136), (3, 384, 1000), (7, 1152, 576), (15, 2048, 4096), (16, 2048, 264),
+    (17, 640, 1048), (31, 4096, 120), (48, 2048, 1024), (63, 896, 392), (64, 1408, 512), (65, 1408, 512), (80, 512, 2112),
+    (97, 768, 2048), (127, 1024, 640), (128, 1024, 640), (129, 1024, 640), (200, 7168, 576), (255, 384, 1528), (256, 2048, 1024),
+    (257, 2048, 1000), (333, 7168, 1584), (511, 1024, 2048), (513, 640, 1160), (1000, 2048, 1544), (2049, 1280, 1152), (4096, 512, 4096),
+]
+
+
+@pytest.mark.parametrize("T,K,N", SHAPES)
+def test_linear(T, K, N):
+    xq, xs = quant(rows(T, K, T + K))
+    w, ws = weight(N, K, N)
+    out = fg().fp8_block_linear(xq, w, ws, x_scale=xs)
+    assert out.shape == (T, N) and out.dtype == torch.bfloat16
+    check(out, values(xq, xs), weight_values(w, ws))
+    again = fg().fp8_block_linear(xq, w, ws, x_scale=xs)
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16)), "the result depends on timing"
+    status()
+
+
+@pytest.mark.parametrize("T,K,N", [(1, 256, 64), (5, 2048, 392), (70, 1024, 1000), (300, 896, 1544)])
+@pytest.mark.parametrize("bias", [None, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("addend", [False, True])
+@pytest.mark.parametrize("x_dtype", ["bf16", "e4m3"])
+def test_linear_extras_and_inputs(T, K, N, bias, addend, x_dtype):
+    x = rows(T, K, 5).bfloat16()
+    xq, xs = quant(x)
+    w, ws = weight(N, K, 6)
+    b = None if bias is None else torch.randn(N, generator=gen(7), device="cuda").to(bias)
+    a = torch.randn(T, N, generator=gen(8), device="cuda").bfloat16() if addend else None
+    more = (0 if b is None else b.double()) + (torch.zeros(T, N, device="cuda").double() if a is None else a.double())
+    args = dict(x=x) if x_dtype == "bf16" else dict(x=xq, x_scale=xs)
+    keep = None if a is None else a.clone()
+    check(fg().fp8_block_linear(w=w, w_scale=ws, bias=b, addend=a, **args), values(xq, xs), weight_values(w, ws), more)
+    assert a is None or torch.equal(a, keep)
+    status()
+
+
+def gate_up(xq, xs, w, ws, activation):
+    """The first half of the MLP through its own entry point: (q, scale)."""
+    from flaggems_sglang_b200 import _C
+
+    T, K = xq.shape
+    I = w.shape[0] // 2
+    q = torch.empty(T, I, dtype=torch.float8_e4m3fn, device="cuda")
+    s = torch.empty(T, I // GROUP, dtype=torch.float32, device="cuda")
+    _C.check(_C.lib().fmoe_fp8_gate_up(_C.Fp8Args(
+        x_dtype=_C.E4M3, activation=_C.ACTIVATIONS[activation], T=T, K=K, I=I, x=xq.data_ptr(), x_scale=xs.data_ptr(), w=w.data_ptr(),
+        w_scale=ws.data_ptr(), out=q.data_ptr(), out_scale=s.data_ptr()), _C.stream_ptr()))
+    return q, s
+
+
+MLP_SHAPES = [(1, 128, 128, 8), (1, 7168, 2048, 7168), (4, 2048, 768, 2048), (16, 512, 384, 136), (33, 1152, 256, 1000), (64, 1024, 512, 512),
+              (65, 1024, 512, 512), (97, 2048, 768, 2048), (128, 640, 1408, 264), (200, 896, 640, 1160), (555, 1024, 2048, 1024),
+              (1030, 2048, 768, 2048)]
+
+
+@pytest.mark.parametrize("T,K,I,N", MLP_SHAPES)
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_gated_mlp(T, K, I, N, activation):
+    xq, xs = quant(rows(T, K, 11, wide=False))
+    w13, s13 = weight(2 * I, K, 12)
+    w2, s2 = weight(N, I, 13)
+    xv, wv = values(xq, xs), weight_values(w13, s13)
+    gate, up = (xv @ wv.t()).chunk(2, dim=1)
+    eg, eu = ((xv.abs() @ wv.abs().t()) * sum_error(K)).chunk(2, dim=1)
+    h = (torch.nn.functional.silu(gate) if activation == "silu" else torch.nn.functional.gelu(gate)) * up
+    # |act(g)| <= |g| and |act'| < 1.13: what the sums' errors do to h, and 2^-20 for exp, erf and division of the activation
+    eh = 1.13 * eg * (up.abs() + eu) + gate.abs() * eu + h.abs() * 2.0 ** -20 + (1.13 * gate.abs() * up.abs()) * 2.0 ** -22
+    q, s = gate_up(xq, xs, w13, s13, activation)
+    # scale: of the group's largest magnitude; value: half a step of e4m3, 2^-4 of it or 2^-10 (subnormal) times the scale
+    top, top_e = (z.view(T, I // GROUP, GROUP).abs().amax(-1) for z in (h, eh))
+    want = top.clamp_min(1e-10) / 448
+    assert ((s.double() - want).abs() <= top_e / 448 + want * 2.0 ** -23).all()
+    sv = s.double().repeat_interleave(GROUP, 1)
+    off = (q.double() * sv - h).abs()
+    assert (off <= (h.abs() + eh) * 2.0 ** -4 + sv * 2.0 ** -10 + eh + h.abs() * 2.0 ** -22 + sv * 448 * 2.0 ** -22).all()
+    out = fg().fp8_gated_mlp(xq, w13, s13, w2, s2, x_scale=xs, activation=activation)
+    check(out, values(q, s), weight_values(w2, s2))
+    add = torch.randn(T, N, generator=gen(14), device="cuda").bfloat16()
+    check(fg().fp8_gated_mlp(xq, w13, s13, w2, s2, x_scale=xs, activation=activation, addend=add), values(q, s), weight_values(w2, s2), add)
+    status()
+
+
+def test_gated_mlp_of_bf16_rows_is_that_of_their_quantised_form():
+    for T in (1, 50, 140):
+        x = rows(T, 1024, 21).bfloat16()
+        xq, xs = quant(x)
+        w13, s13 = weight(512, 1024, 22)
+        w2, s2 = weight(1024, 256, 23)
+        a = fg().fp8_gated_mlp(x, w13, s13, w2, s2)
+        b = fg().fp8_gated_mlp(xq, w13, s13, w2, s2, x_scale=xs)
+        assert torch.equal(a, b)
+    status()
+
+
+def test_rows_do_not_depend_on_their_neighbours():
+    """A row with NaN or infinity in it, or of zeros, leaves the other rows' bits alone; the rows behind the last are not there."""
+    T, K, N = 37, 1024, 520
+    xq, xs = quant(rows(T, K, 31))
+    w, ws = weight(N, K, 32)
+    clean = fg().fp8_block_linear(xq, w, ws, x_scale=xs)
+    bad, bad_s = xq.clone(), xs.clone()
+    bad.view(torch.uint8)[5, 100] = 0x7F  # NaN
+    bad_s[9, 3] = float("inf")
+    bad.view(torch.uint8)[12] = 0
+    got = fg().fp8_block_linear(bad, w, ws, x_scale=bad_s)
+    assert torch.isnan(got[5]).all() and not torch.isfinite(got[9]).any() and (got[12] == 0).all()
+    keep = [t for t in range(T) if t not in (5, 9, 12)]
+    assert torch.equal(got[keep], clean[keep])
+    status()
+
+
+def test_output_rows_behind_the_last_are_left_alone():
+    """Through the C entry point, into a buffer with rows behind the last token's and a neighbour in front."""
+    from flaggems_sglang_b200 import _C
+
+    T, K, N = 21, 512, 200
+    xq, xs = quant(rows(T, K, 41))
+    w, ws = weight(N, K, 42)
+    buf = torch.full((T + 20, N), 7.0, dtype=torch.bfloat16, device="cuda")
+    _C.check(_C.lib().fmoe_fp8_linear(_C.Fp8Args(x_dtype=_C.E4M3, T=T, K=K, N=N, x=xq.data_ptr(), x_scale=xs.data_ptr(), w=w.data_ptr(),
+                                                 w_scale=ws.data_ptr(), out=buf[10:].data_ptr()), _C.stream_ptr()))
+    assert (buf[:10] == 7).all() and (buf[10 + T:] == 7).all()
+    assert torch.equal(buf[10:10 + T], fg().fp8_block_linear(xq, w, ws, x_scale=xs))
+    status()
+
+
+def test_strided_and_misaligned_inputs():
+    T, K, N = 19, 512, 320
+    big = rows(T, 2 * K, 51).bfloat16()
+    x = big[:, K:]
+    w, ws = weight(N, K, 52)
+    want = fg().fp8_block_linear(x.contiguous(), w, ws)
+    assert torch.equal(fg().fp8_block_linear(x, w, ws), want)
+    odd = torch.empty(T * K + 1, dtype=torch.bfloat16, device="cuda")[1:].view(T, K)
+    odd.copy_(x)
+    assert odd.data_ptr() % 16
+    assert torch.equal(fg().fp8_block_linear(odd, w, ws), want)
+    wo = torch.empty(N * K + 3, dtype=torch.float8_e4m3fn, device="cuda")[3:].view(N, K)
+    wo.copy_(w)
+    assert torch.equal(fg().fp8_block_linear(x, wo, ws.t().contiguous().t()), want)
+
+
+def test_empty_batch():
+    w, ws = weight(256, 512, 61)
+    w2, s2 = weight(512, 128, 62)
+    for x in (torch.empty(0, 512, dtype=torch.bfloat16, device="cuda"),):
+        assert fg().fp8_block_linear(x, w, ws).shape == (0, 256)
+        assert fg().fp8_gated_mlp(x, w, ws, w2, s2).shape == (0, 512)
+
+
+def test_graphs_and_streams():
+    """Captured calls replayed with new inputs, two graphs in turn, and calls on two streams at once give what eager calls give."""
+    T, K, I, N = 24, 1024, 512, 1024
+    w13, s13 = weight(2 * I, K, 71)
+    w2, s2 = weight(N, I, 72)
+    inputs = [rows(T, K, 73 + i, wide=False).bfloat16() for i in range(3)]
+    want = [fg().fp8_gated_mlp(x, w13, s13, w2, s2) for x in inputs]
+    graphs = []
+    for _ in range(2):
+        x = inputs[0].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            fg().fp8_gated_mlp(x, w13, s13, w2, s2)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = fg().fp8_gated_mlp(x, w13, s13, w2, s2)
+        graphs.append((g, x, y))
+    for i in (1, 2, 0):
+        for g, x, y in graphs:
+            x.copy_(inputs[i])
+            g.replay()
+        for g, x, y in graphs:
+            assert torch.equal(y, want[i])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for s in range(2):
+            with torch.cuda.stream(streams[s]):
+                got[s].append(fg().fp8_gated_mlp(inputs[s], w13, s13, w2, s2))
+    torch.cuda.synchronize()
+    for s in range(2):
+        for y in got[s]:
+            assert torch.equal(y, want[s])
+    status()
+
+
+def test_refusals():
+    w, ws = weight(256, 512, 81)
+    x = torch.zeros(4, 512, dtype=torch.bfloat16, device="cuda")
+    xq, xs = quant(x)
+    lin = fg().fp8_block_linear
+    for bad in (dict(x=x[None]), dict(x=x.half()), dict(x=x[:, :500]), dict(x=xq), dict(x=xq, x_scale=xs.double()), dict(x=xq, x_scale=xs[:3]),
+                dict(x=x, x_scale=xs), dict(w=w.float()), dict(w=w[:, :384]), dict(w=w[:4], w_scale=ws[:1]), dict(w_scale=ws[:1]),
+                dict(w_scale=ws.double()), dict(bias=torch.zeros(255, device="cuda")), dict(bias=torch.zeros(256, dtype=torch.int32, device="cuda")),
+                dict(addend=torch.zeros(4, 256, device="cuda")), dict(addend=torch.zeros(3, 256, dtype=torch.bfloat16, device="cuda"))):
+        with pytest.raises(ValueError):
+            lin(**{**dict(x=x, w=w, w_scale=ws), **bad})
+    with pytest.raises(RuntimeError):
+        lin(x.cpu(), w, ws)
+    w2, s2 = weight(512, 128, 82)
+    mlp = fg().fp8_gated_mlp
+    for bad in (dict(activation="relu"), dict(w2=w2[:, :64]), dict(w13=w[:200]), dict(w13=w[:128], w13_scale=ws[:1]), dict(w2_scale=s2[:2]),
+                dict(w2=w2[:4], w2_scale=s2[:1])):
+        with pytest.raises(ValueError):
+            mlp(**{**dict(x=x, w13=w, w13_scale=ws, w2=w2, w2_scale=s2), **bad})

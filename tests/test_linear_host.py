@@ -1,0 +1,99 @@
+"""Refusals and workspaces of the dense e4m3 products and the norm, on the host: nothing is launched."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def C():
+    import __graft_entry__ as ge
+
+    ge.build()
+    from flaggems_sglang_b200 import _C
+
+    return _C
+
+
+def test_struct_layout(C):
+    assert ctypes.sizeof(C.Fp8Args) == 4 * 4 + 4 * 8 + 11 * 8 + 8
+    assert C.Fp8Args.T.offset == 16 and C.Fp8Args.x.offset == 48 and C.Fp8Args.workspace_bytes.offset == 136
+    assert C.Fp8Args().struct_size == ctypes.sizeof(C.Fp8Args)
+
+
+def bad_args(C, entry, **kw):
+    a = C.Fp8Args(**{**dict(x_dtype=C.E4M3, T=3, K=256, N=128, I=128), **kw})
+    rc = getattr(C.lib(), entry)(a, None)
+    return rc, C.lib().fmoe_last_error().decode()
+
+
+@pytest.mark.parametrize("entry", ["fmoe_fp8_linear", "fmoe_fp8_gate_up", "fmoe_fp8_mlp"])
+@pytest.mark.parametrize("kw,says", [
+    (dict(x_dtype=0), "bf16 or e4m3"), (dict(T=-1), "bad sizes"), (dict(K=0), "bad sizes"), (dict(K=200), "multiple of 128"),
+    (dict(T=1 << 31), "too large"), (dict(T=1 << 29, N=1 << 28, I=1 << 28), "too large"), (dict(), "null")])
+def test_products_refuse(C, entry, kw, says):
+    rc, msg = bad_args(C, entry, **kw)
+    assert rc == C.ERR_INVALID_ARG and says in msg, msg
+    assert entry.split("fmoe_")[1] in msg
+
+
+def test_products_refuse_widths_and_activations(C):
+    assert "multiple of 8" in bad_args(C, "fmoe_fp8_linear", N=12)[1]
+    assert "multiple of 128" in bad_args(C, "fmoe_fp8_gate_up", I=64)[1]
+    assert "multiple of 128" in bad_args(C, "fmoe_fp8_mlp", I=64)[1]
+    assert "multiple of 8" in bad_args(C, "fmoe_fp8_mlp", N=12)[1]
+    assert "activation" in bad_args(C, "fmoe_fp8_mlp", activation=2)[1]
+    a = C.Fp8Args(x_dtype=C.E4M3, T=3, K=256, N=128)
+    a.struct_size -= 8
+    assert C.lib().fmoe_fp8_linear(a, None) == C.ERR_INVALID_ARG and b"struct_size" in C.lib().fmoe_last_error()
+    assert C.lib().fmoe_fp8_linear(None, None) == C.ERR_INVALID_ARG
+
+
+def test_misaligned_pointers_and_small_workspaces(C):
+    ok = dict(x=4096, x_scale=4096, w=4096, w_scale=4096, out=4096)
+    for name in ("x", "w", "out", "bias", "addend"):
+        rc, msg = bad_args(C, "fmoe_fp8_linear", **{**ok, name: 4104})
+        assert rc == C.ERR_INVALID_ARG and "misaligned" in msg, (name, msg)
+    assert "x_scale" in bad_args(C, "fmoe_fp8_linear", **{**ok, "x_scale": None})[1]
+    a = C.Fp8Args(x_dtype=C.BF16, T=3, K=256, N=128, I=384, w2=4096, w2_scale=4096, **ok)
+    lib = C.lib()
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    assert lib.fmoe_fp8_linear_workspace_bytes(a) == up(3 * 256) + up(3 * 2 * 4) == lib.fmoe_fp8_gate_up_workspace_bytes(a)
+    need = lib.fmoe_fp8_mlp_workspace_bytes(a)
+    assert need == up(3 * 256) + up(3 * 2 * 4) + up(3 * 384) + up(3 * 3 * 4)
+    for ws, size in ((None, need), (4096, need - 1), (4096 + 128, need)):
+        a.workspace, a.workspace_bytes = ws, size
+        assert lib.fmoe_fp8_mlp(a, None) == C.ERR_INVALID_ARG and b"workspace" in lib.fmoe_last_error()
+    a.x_dtype = C.E4M3
+    assert lib.fmoe_fp8_linear_workspace_bytes(a) == 0
+    a.K = 100
+    assert lib.fmoe_fp8_linear_workspace_bytes(a) < 0
+
+
+def test_no_tokens_is_no_work(C):
+    for entry in ("fmoe_fp8_linear", "fmoe_fp8_gate_up", "fmoe_fp8_mlp"):
+        assert bad_args(C, entry, T=0)[0] == C.OK
+
+
+def test_norm_refuses(C):
+    def call(x=4096, xs=256, r=None, rs=256, dtype=1, w=4096, wd=1, rows=2, K=256, eps=1e-6, tok=0, q=4096, s=4096, n=None):
+        rc = C.lib().fmoe_rms_norm_quant(x, xs, r, rs, dtype, w, wd, rows, K, eps, tok, q, s, n, None)
+        return rc, C.lib().fmoe_last_error().decode()
+
+    for kw, says in ((dict(dtype=2), "x must be"), (dict(wd=2), "weight"), (dict(K=200), "multiple of 128"), (dict(K=204, tok=1), "multiple of 8"),
+                     (dict(K=16512, xs=16512), "16384"), (dict(rows=-1), "rows"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(xs=255), "strides"),
+                     (dict(xs=260), "strides"), (dict(r=4096, rs=128), "strides"), (dict(x=None), "null"), (dict(q=None), "null"),
+                     (dict(x=4100), "misaligned"), (dict(r=4104), "misaligned"), (dict(n=4104), "misaligned"), (dict(q=4100), "misaligned")):
+        rc, msg = call(**kw)
+        assert rc == C.ERR_INVALID_ARG and says in msg, (kw, msg)
+    assert call(rows=0, x=None)[0] == C.OK
+
+
+def test_ops_refuse_cpu_tensors():
+    import flaggems_sglang_b200 as fg
+
+    x, w = torch.zeros(2, 256, dtype=torch.bfloat16), torch.zeros(128, 256).to(torch.float8_e4m3fn)
+    for call in (lambda: fg.rms_norm_quant_fp8(x, torch.ones(256)), lambda: fg.fp8_block_linear(x, w, torch.ones(1, 2)),
+                 lambda: fg.fp8_gated_mlp(x, w, torch.ones(1, 2), w, torch.ones(1, 2))):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
