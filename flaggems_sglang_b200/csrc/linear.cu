@@ -5,21 +5,29 @@
 // The tensor cores cannot apply a scale inside their accumulator that changes with K, so every K block of 128 is multiplied into
 // a fresh TMEM partial (4 MMAs of K = 32) which the fold warps add, times a[t, kb] * b[n / 128, kb], to sums in registers.
 //
-//   tile    : 128 weight rows (gate/up: 128 gate rows and the same 128 up rows) on the MMA's M side x up to 64 or 128 tokens on N.
-//             With the weights on M a call of one token costs a 16-column tile
+//   tile    : 128 weight rows (gate/up: 128 gate rows and the same 128 up rows) on the MMA's M side x up to 16, 32, 64 or 128 tokens on
+//             N.  With the weights on M a call of one token costs a 16-column tile
 //   split   : S CTAs of a cluster share a tile, each with a contiguous part of its K blocks, so that few tiles still fill the
 //             chip.  Their sums meet through distributed shared memory, added in the order of the CTAs: the result does not
 //             depend on timing, and there is no scratch in global memory and no counter
-//   warps   : fold warps (four per 128 rows x 64 tokens: TMEM lane quarter = warp % 4, 64 sums per thread), then TMA, MMA, and
-//             two that multiply token and weight scales into a ring of factors
+//   warps   : fold warps (TMEM lane quarter = warp % 4; 16 to 64 sums per thread), then TMA, MMA, and two that multiply token and weight
+//             scales into a ring of factors
+//   batches : up to 32 tokens the partials of two or four K blocks are handed to the fold together.  What a K block costs there is not
+//             its FMAs but the chain wait - TMEM read - wait - hand back: 400 SM cycles each alone, 180 in batches of four (one token,
+//             7168 x 2048: 5.4 -> 4.9 us, gate/up of 7168 x 2 x 2048 10.5 -> 7.5 us)
 //   epilogue: sums to shared memory [token][row], then a warp per token: a row of 128 channels is one coalesced store, and for
 //             gate/up it is one quantisation group, whose largest magnitude is a warp reduction
+// Two CTAs per SM for plain products of up to 32 tokens: twice as many clusters of 8 fit.  (Gate/up has eight fold warps; with two CTAs of
+// 384 threads an SM leaves 80 registers, and the fold takes twice as long as with one CTA and 141.)
 // Every mbarrier wait is bounded; the cluster barriers are reached by every thread on every path.
+// What bounds it: up to 64 tokens HBM beside the launch, the first loads and the join (one token, 7168 x 4096: 6.2 us, 4.7 TB/s); with 128
+// tokens what an SM takes in from L2, 32 KB per K block.
 #include "linear.cuh"
 #include "pair.cuh"
 #include "rows.cuh"
 
 #include <algorithm>
+#include <mutex>
 
 namespace fmoe {
 
@@ -30,25 +38,33 @@ namespace {
 
 constexpr int KBYTES = 128;
 constexpr int W_BYTES = 128 * KBYTES;
-constexpr int kMaxSmem = 227 * 1024;
 constexpr int kMaxStages = 12;
 constexpr int kGroup = 8;  // K blocks per factor slot
 constexpr int kSlots = 4;
+constexpr int kMaxSplit = 8;
 constexpr int BAR_BYTES = 512;
 
-// HALVES: 1 = plain, 2 = gate rows and up rows; COLS: most tokens of a tile
-template <int HALVES, int COLS>
+// HALVES: 1 = plain, 2 = gate rows and up rows; COLS: most tokens of a tile; BATCH: K blocks whose partials are handed to the fold
+// together; ACC: sums per fold thread; CTAS: CTAs per SM
+template <int HALVES_, int COLS_, int BATCH_, int ACC_, int CTAS_>
 struct Geo {
-  static constexpr int FOLD_WARPS = 4 * HALVES * (COLS / 64);
+  static constexpr int HALVES = HALVES_, COLS = COLS_, BATCH = BATCH_, ACC = ACC_, CTAS = CTAS_;
+  static constexpr int FOLD_WARPS = 4 * HALVES * (COLS / ACC);
   static constexpr int THREADS = (FOLD_WARPS + 4) * 32;
-  static constexpr int BUF_COLS = HALVES * COLS;
-  static constexpr int BUFS = 512 / BUF_COLS < 4 ? 512 / BUF_COLS : 4;
+  static constexpr int HALF_COLS = BATCH * COLS;        // TMEM columns of one half's partials
+  static constexpr int BUF_COLS = HALVES * HALF_COLS;
+  static constexpr int BUFS = 512 / CTAS / BUF_COLS < 4 ? 512 / CTAS / BUF_COLS : 4;
   static constexpr int TMEM_COLS = BUFS * BUF_COLS;
-  static constexpr int KB_FLOATS = HALVES * COLS;  // factors of one K block
+  static constexpr int STAGED = ACC > 32 ? 16 : BATCH * ACC;  // columns read from TMEM before the first is added
+  static constexpr int KB_FLOATS = HALVES * COLS;       // factors of one K block
   static constexpr int SLOT_FLOATS = kGroup * KB_FLOATS;
   static constexpr int FIXED_BYTES = BAR_BYTES + kSlots * SLOT_FLOATS * 4;
+  // what a CTA takes, whatever its ring needs: so that neither a third CTA nor another TMEM kernel fits beside these, whose TMEM
+  // allocation would wait for this one's end while a cluster of its own waits for it
+  static constexpr int SMEM_BYTES = CTAS == 1 ? 227 * 1024 : 113 * 1024;
   static constexpr int ROWS = 128 * HALVES;
-  static constexpr int SUM_BYTES = COLS * ROWS * 4;  // the sums, in place of the ring
+  static constexpr int SUM_BYTES = COLS * ROWS * 4;     // the sums, in place of the ring
+  static_assert(SUM_BYTES <= SMEM_BYTES - FIXED_BYTES && TMEM_COLS * CTAS <= 512 && kGroup % BATCH == 0, "shared memory, TMEM");
 };
 
 struct KernelParams {
@@ -73,13 +89,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity));
 }
 
-template <int HALVES, int COLS>
-__global__ void __launch_bounds__(Geo<HALVES, COLS>::THREADS, 1)
+template <typename G>
+__global__ void __launch_bounds__(G::THREADS, G::CTAS)
 fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const KernelParams p) {
-  using G = Geo<HALVES, COLS>;
+  constexpr int HALVES = G::HALVES, COLS = G::COLS, BATCH = G::BATCH;
   extern __shared__ __align__(1024) uint8_t smem[];
   // barriers and factors first in the fixed part behind the ring; the ring itself starts at 0 (1024-byte aligned stages)
-  uint8_t* fixed = smem + kMaxSmem - G::FIXED_BYTES;
+  uint8_t* fixed = smem + G::SMEM_BYTES - G::FIXED_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
   uint64_t* full_bar = bars;                    // [stages] TMA -> MMA
   uint64_t* empty_bar = bars + kMaxStages;      // [stages] MMA -> TMA
@@ -187,26 +203,27 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       const uint32_t idesc = ptx::make_idesc(/*e4m3*/ 0, 128, (uint32_t)p.token_tile);
       int stage = 0;
       uint32_t phase = 0;
-      for (int step = 0; step < kb1 - kb0; ++step) {
-        const int buf = step % G::BUFS;
+      const int steps = kb1 - kb0;
+      for (int step = 0; step < steps; ++step) {
+        const int batch = step / BATCH, buf = batch % G::BUFS;
         if (!ptx::mbar_wait(&full_bar[stage], phase)) {
           report(0x1200 | stage);
           break;
         }
-        if (!ptx::mbar_wait(&part_empty[buf], ((step / G::BUFS) & 1) ^ 1)) {
+        if (step % BATCH == 0 && !ptx::mbar_wait(&part_empty[buf], ((batch / G::BUFS) & 1) ^ 1)) {
           report(0x1240 | buf);
           break;
         }
         ptx::tc_fence_after_sync();
         const uint64_t off = (uint64_t)(stage * (p.stage_bytes >> 4));
+        const uint32_t to = tmem_base + buf * G::BUF_COLS + step % BATCH * COLS;
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
 #pragma unroll
           for (int kk = 0; kk < KBYTES / 32; ++kk)
-            ptx::mma_f8f6f4_ss(tmem_base + buf * G::BUF_COLS + h * COLS, dw0 + off + h * (W_BYTES >> 4) + 2 * kk, dx0 + off + 2 * kk,
-                               idesc, kk != 0);
+            ptx::mma_f8f6f4_ss(to + h * G::HALF_COLS, dw0 + off + h * (W_BYTES >> 4) + 2 * kk, dx0 + off + 2 * kk, idesc, kk != 0);
         }
-        ptx::mma_commit(&part_full[buf]);
+        if (step % BATCH == BATCH - 1 || step == steps - 1) ptx::mma_commit(&part_full[buf]);
         ptx::mma_commit(&empty_bar[stage]);
         if (++stage == p.stages) {
           stage = 0;
@@ -221,9 +238,15 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     const int me = warp - (G::FOLD_WARPS + 2);
     for (int g = me; g * kGroup < kb1 - kb0; g += 2) {
       const int first = kb0 + g * kGroup, count = min(kGroup, kb1 - first), slot = g % kSlots;
-      float a[COLS / 32][kGroup];
+      constexpr int PER_LANE = (COLS + 31) / 32;
+      float a[PER_LANE][kGroup], b[HALVES][kGroup];
 #pragma unroll
-      for (int j = 0; j < COLS / 32; ++j) {
+      for (int h = 0; h < HALVES; ++h) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) b[h][i] = i < count ? __ldg(p.w_scale + (int64_t)(h ? up_tile : row_tile) * p.kblocks + first + i) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < PER_LANE; ++j) {
         const int64_t t = tok0 + lane + 32 * j;
 #pragma unroll
         for (int i = 0; i < kGroup; ++i)
@@ -236,13 +259,11 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       float* dst = factors + slot * G::SLOT_FLOATS + lane;
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) {
-        if (i < count) {
 #pragma unroll
-          for (int h = 0; h < HALVES; ++h) {
-            const float b = __ldg(p.w_scale + (int64_t)(h ? up_tile : row_tile) * p.kblocks + first + i);
+        for (int h = 0; h < HALVES; ++h) {
 #pragma unroll
-            for (int j = 0; j < COLS / 32; ++j) dst[(i * HALVES + h) * COLS + 32 * j] = a[j][i] * b;
-          }
+          for (int j = 0; j < PER_LANE; ++j)
+            if (COLS % 32 == 0 || lane < COLS) dst[(i * HALVES + h) * COLS + 32 * j] = a[j][i] * b[h][i];
         }
       }
       __syncwarp();
@@ -251,55 +272,67 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   } else {
     // ---------------- fold ----------------
     pdl_entry_late();
-    const int piece = warp >> 2, half = piece / (COLS / 64), col0 = piece % (COLS / 64) * 64;
-    const int cols = min(64, p.token_tile - col0);  // a multiple of 16, or nothing
-    const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * COLS + col0;
-    float acc[64];
+    constexpr int ACC = G::ACC, STAGED = G::STAGED;
+    const int piece = warp >> 2, half = piece / (COLS / ACC), col0 = piece % (COLS / ACC) * ACC;
+    const int cols = min(ACC, p.token_tile - col0);  // a multiple of 16, or nothing
+    const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * G::HALF_COLS + col0;
+    float acc[ACC];
 #pragma unroll
-    for (int i = 0; i < 64; ++i) acc[i] = 0.f;
+    for (int i = 0; i < ACC; ++i) acc[i] = 0.f;
     const int steps = kb1 - kb0;
-    for (int step = 0; step < steps; ++step) {
-      const int buf = step % G::BUFS, g = step / kGroup, slot = g % kSlots;
+    for (int step = 0; step < steps; step += BATCH) {
+      const int batch = step / BATCH, buf = batch % G::BUFS, g = step / kGroup, slot = g % kSlots, blocks = min(BATCH, steps - step);
       if (step % kGroup == 0 && !warp_wait(&sc_full[slot], (g / kSlots) & 1)) {
         report(0x1400 | slot);
         break;
       }
-      if (!warp_wait(&part_full[buf], (step / G::BUFS) & 1)) {
+      if (!warp_wait(&part_full[buf], (batch / G::BUFS) & 1)) {
         report(0x1440 | buf);
         break;
       }
       ptx::tc_fence_after_sync();
-      const float4* f4 = reinterpret_cast<const float4*>(factors + slot * G::SLOT_FLOATS + ((step % kGroup) * HALVES + half) * COLS + col0);
+      const float4* f4 = reinterpret_cast<const float4*>(factors + slot * G::SLOT_FLOATS + (step % kGroup * HALVES + half) * COLS + col0);
+      // The batch's columns, ACC of each K block in turn.  As many as registers allow are read before the first is waited for, and the
+      // partials are handed back before the FMAs: the MMAs of later K blocks run beside them.
+      constexpr int ALL = BATCH * ACC;
+      auto tok = [](int q) { return q % ACC; };
+      auto block = [](int q) { return q / ACC; };
+      auto there = [&](int q) { return block(q) < blocks && tok(q) < cols; };
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (16 * c < cols) {
-          uint32_t v[16];
-          ptx::tmem_ld_32x32b_x16(from + buf * G::BUF_COLS + 16 * c, v);
-          float4 f[4];
+      for (int c = 0; c < ALL; c += STAGED) {
+        uint32_t v[STAGED];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) f[q] = f4[4 * c + q];
-          ptx::tmem_ld_wait();
+        for (int q = 0; q < STAGED; q += 16)
+          if (there(c + q))
+            ptx::tmem_ld_32x32b_x16(from + buf * G::BUF_COLS + block(c + q) * COLS + tok(c + q), *reinterpret_cast<uint32_t(*)[16]>(v + q));
+        ptx::tmem_ld_wait();
+        if (c + STAGED >= ALL) {
+          ptx::tc_fence_before_sync();
+          __syncwarp();
+          ptx::mbar_arrive_if(lane == 0, &part_empty[buf]);
+        }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            acc[16 * c + 4 * q] = fmaf(__uint_as_float(v[4 * q]), f[q].x, acc[16 * c + 4 * q]);
-            acc[16 * c + 4 * q + 1] = fmaf(__uint_as_float(v[4 * q + 1]), f[q].y, acc[16 * c + 4 * q + 1]);
-            acc[16 * c + 4 * q + 2] = fmaf(__uint_as_float(v[4 * q + 2]), f[q].z, acc[16 * c + 4 * q + 2]);
-            acc[16 * c + 4 * q + 3] = fmaf(__uint_as_float(v[4 * q + 3]), f[q].w, acc[16 * c + 4 * q + 3]);
+        for (int q = 0; q < STAGED; q += 4) {
+          if (there(c + (q & ~15))) {
+            const float4 f = f4[block(c + q) * HALVES * (COLS / 4) + tok(c + q) / 4];
+            float* d = acc + tok(c + q);
+            d[0] = fmaf(__uint_as_float(v[q]), f.x, d[0]);
+            d[1] = fmaf(__uint_as_float(v[q + 1]), f.y, d[1]);
+            d[2] = fmaf(__uint_as_float(v[q + 2]), f.z, d[2]);
+            d[3] = fmaf(__uint_as_float(v[q + 3]), f.w, d[3]);
           }
         }
       }
-      ptx::tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-        ptx::mbar_arrive(&part_empty[buf]);
-        if (step % kGroup == kGroup - 1 || step == steps - 1) ptx::mbar_arrive(&sc_empty[slot]);
+      if (step % kGroup == kGroup - BATCH || step + BATCH >= steps) {
+        __syncwarp();
+        ptx::mbar_arrive_if(lane == 0, &sc_empty[slot]);
       }
     }
     // Sums to shared memory in place of the ring: the last partial is complete, so every MMA has read its operands.  A warp
     // writes 32 consecutive rows of a token.
     float* sums = reinterpret_cast<float*>(smem) + half * 128 + (warp & 3) * 32 + lane;
 #pragma unroll
-    for (int i = 0; i < 64; ++i)
+    for (int i = 0; i < ACC; ++i)
       if (i < cols) sums[(col0 + i) * G::ROWS] = acc[i];
   }
 
@@ -313,100 +346,126 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
 
   // ---------------- epilogue: a warp per token, the tile's tokens dealt to the CTAs of the cluster ----------------
   const int tokens = (int)min((int64_t)p.token_tile, p.T - tok0);
-  const uint32_t sums = ptx::smem_u32(smem) + lane * 16;
-  for (int t = rank + S * warp; t < tokens; t += S * (G::THREADS / 32)) {
-    float4 v[HALVES];
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h) v[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
-        const uint32_t at = sums + (t * G::ROWS + h * 128) * 4;
-        const float4 part = ptx::ld_cluster_f4(S > 1 ? ptx::mapa(at, s) : at);
-        v[h].x += part.x;
-        v[h].y += part.y;
-        v[h].z += part.z;
-        v[h].w += part.w;
-      }
-    }
+  join_tokens<HALVES, kMaxSplit>(rank + S * warp, S * (G::THREADS / 32), tokens, S, 0, 1, ptx::smem_u32(smem) + lane * 16, G::ROWS * 4,
+                                 [&](int t, float(&v)[HALVES][4]) {
     const int64_t row = tok0 + t;
-    const int64_t ch = (int64_t)row_tile * 128 + lane * 4;
     if constexpr (HALVES == 1) {
-      if (ch < p.n) {
-        if (p.bias) {
-          const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + ch));
-          v[0].x += b.x;
-          v[0].y += b.y;
-          v[0].z += b.z;
-          v[0].w += b.w;
-        }
-        if (p.addend) {
-          const uint2 raw = __ldg(reinterpret_cast<const uint2*>(p.addend + row * p.n + ch));
-          const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw);
-          v[0].x += __low2float(e[0]);
-          v[0].y += __high2float(e[0]);
-          v[0].z += __low2float(e[1]);
-          v[0].w += __high2float(e[1]);
-        }
-        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + row * p.n + ch) =
-            make_uint2(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[0].z, v[0].w));
-      }
+      const int64_t ch = (int64_t)row_tile * 128 + lane * 4;
+      if (ch < p.n) store_plain(v[0], p.bias, p.addend, reinterpret_cast<__nv_bfloat16*>(p.out), row * p.n, ch);
     } else {
-      float h[4];
-      h[0] = act_mul_fast(v[0].x, v[1].x, p.activation);
-      h[1] = act_mul_fast(v[0].y, v[1].y, p.activation);
-      h[2] = act_mul_fast(v[0].z, v[1].z, p.activation);
-      h[3] = act_mul_fast(v[0].w, v[1].w, p.activation);
-      float amax = fmaxf(fmaxf(fabsf(h[0]), fabsf(h[1])), fmaxf(fabsf(h[2]), fabsf(h[3])));
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-      const float s = group_scale(amax);
-      *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + row * p.n + ch) = quant4(h, s, __frcp_rn(s), amax <= 3.0e38f);
-      if (lane == 0) p.out_scale[row * (p.n / 128) + row_tile] = s;
+      store_gated(v, p.activation, reinterpret_cast<uint8_t*>(p.out) + row * p.n + row_tile * 128, p.out_scale + row * (p.n / 128) + row_tile);
     }
-  }
+  });
   if (S > 1) ptx::cluster_sync_all();  // nobody leaves while its sums are read
 }
 
-// CTAs that share a tile's K blocks.  The time of a launch as a model: rounds of CTAs, each with a fixed part (launch, first
-// loads, sums) and its K blocks at the slowest of HBM's share, what one SM takes in from L2, and the fold.
-int pick_split(int64_t tiles, int kblocks, int halves, int cols, int sms) {
-  int best = 1;
+// Clusters of 1 to 8 CTAs that the device holds at a time, by the CTAs per SM.  GPCs have different numbers of SMs, so that clusters of
+// 7 or 8 leave a fifth of them idle where a CTA takes a whole SM.
+struct Residents {
+  int n[2][kMaxSplit + 1];
+};
+
+const Residents& residents() {
+  static std::mutex mu;
+  static Residents known[kMaxDevices];
+  static bool done[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) dev = 0;
+  std::lock_guard<std::mutex> lock(mu);
+  Residents& r = known[dev];
+  if (!done[dev]) {
+    auto ask = [](const void* kernel, int threads, int smem, int split) {
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(split);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = split;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0) return n;
+      cudaGetLastError();
+      return 0;
+    };
+    for (int s = 1; s <= kMaxSplit; ++s) {
+      using One = Geo<1, 64, 1, 32, 1>;
+      using Two = Geo<1, 16, 4, 16, 2>;
+      r.n[0][s] = ask((const void*)fp8_linear_kernel<One>, One::THREADS, One::SMEM_BYTES, s);
+      r.n[1][s] = ask((const void*)fp8_linear_kernel<Two>, Two::THREADS, Two::SMEM_BYTES, s);
+      for (int c = 0; c < 2; ++c)
+        if (r.n[c][s] == 0) r.n[c][s] = std::max(1, 148 * (c + 1) / s);
+    }
+    done[dev] = true;
+  }
+  return r;
+}
+
+// The kernel and the number of CTAs (pair kernel: pairs) that share a tile's K blocks, by what the launch should take.  The models were
+// fitted to launches of K = 2048, 4096 and 7168, N = 512 to 7168 (gate/up: I = 768 to 3584) and 1 to 1024 tokens with every split; us:
+//   one CTA    rounds of clusters, each its K blocks at the slowest of the fold (0.18 to 0.95 by width), HBM's share of the weights and
+//              what an SM and the chip take in from L2, an epilogue, and the join of the sums
+//   CTA pairs  rounds of 0.38 per K block and the epilogue; shared tiles 0.44 and a longer one, as all sums cross shared memory
+struct Choice {
+  bool pair;
+  int split;
+};
+
+Choice choose(const LinearParams& g, bool gated) {
+  const Residents& r = residents();
+  const int halves = gated ? 2 : 1, kblocks = (int)(g.k / 128);
+  const int cols = g.T <= 16 ? 16 : (g.T <= 32 ? 32 : (g.T <= 64 ? 64 : 128));
+  const int ctas = !gated && cols <= 32 ? 2 : 1;
+  const int64_t token_tiles = ceil_div<int64_t>(g.T, cols), tiles = ceil_div<int64_t>(g.n, 128) * token_tiles;
+  const double tokens = (double)(ceil_div<int64_t>(ceil_div<int64_t>(g.T, token_tiles), 16) * 16);
+  const double fold = cols == 128 ? (gated ? 0.31 + 0.005 * tokens : 0.28 + 0.0009 * tokens)
+                                  : (gated ? 0.24 + 0.003 * cols : 0.15 + 0.002 * cols);
+  const double bytes = halves * W_BYTES + tokens * KBYTES;
+  Choice best{false, 1};
   double best_us = 1e30;
-  for (int s = 1; s <= 8 && s <= kblocks; ++s) {
-    const double ctas = (double)tiles * s, rounds = (double)ceil_div<int64_t>(tiles * s, sms);
-    const double active = ctas < sms ? ctas : sms;
-    const double hbm = active * halves * W_BYTES / 6.5e6, l2 = (halves * W_BYTES + cols * KBYTES) / 1.0e5;
-    const double fold = (cols <= 64 ? 0.16 : 0.27) * halves;
-    const double per_block = std::max(hbm, std::max(l2, fold));
-    const double us = rounds * (ceil_div(kblocks, s) * per_block + 2.0 + (s > 1 ? 0.5 + 0.1 * s : 0.0));
+  auto offer = [&](bool pair, int split, double us) {
     if (us < best_us) {
       best_us = us;
-      best = s;
+      best = {pair, split};
     }
+  };
+  for (int s = 1; s <= kMaxSplit && s <= kblocks; ++s) {
+    const int64_t at_once = r.n[ctas - 1][s], rounds = ceil_div<int64_t>(tiles, at_once);
+    const double active = (double)std::min<int64_t>(tiles, at_once) * s, per_sm = std::max(1.0, active / 148);
+    const double hbm = active * halves * W_BYTES / 8.0e6, l2 = std::max(bytes * per_sm / 1.0e5, active * bytes / 1.1e7);
+    const double per_block = std::max(std::max(hbm, l2), fold * per_sm);
+    const double join = s == 1 ? 0.0 : (gated ? 0.4 + 0.1 * s + 0.022 * tokens : 0.2 + 0.05 * s + 0.013 * tokens);
+    offer(false, s, 2.0 + rounds * (0.7 + 0.01 * tokens * halves + ceil_div(kblocks, s) * per_block + join));
+  }
+  if (g.T > 64) {
+    const int64_t pair_tiles = ceil_div<int64_t>(g.T, 256) * ceil_div<int64_t>(g.n, gated ? 128 : 256);
+    offer(true, 1, 3.0 + ceil_div<int64_t>(pair_tiles, r.n[0][2]) * (0.38 * kblocks + (gated ? 2.6 : 4.6)));
+    for (int s = 2; s <= kMaxPairSplit && s <= kblocks; ++s)
+      offer(true, s, 2.8 + ceil_div<int64_t>(pair_tiles, r.n[0][2 * s]) * (0.44 * ceil_div(kblocks, s) + 5.7));
   }
   return best;
 }
 
-template <int HALVES, int COLS>
-int launch(const LinearParams& g, cudaStream_t st) {
-  using G = Geo<HALVES, COLS>;
-  static_assert(G::SUM_BYTES <= kMaxSmem - G::FIXED_BYTES, "shared memory");
-  auto kernel = fp8_linear_kernel<HALVES, COLS>;
+template <typename G>
+int launch(const LinearParams& g, int split, cudaStream_t st) {
+  constexpr int HALVES = G::HALVES, COLS = G::COLS;
+  auto kernel = fp8_linear_kernel<G>;
   static PerDeviceOnce once_attr;
   const cudaError_t attr_err = per_device_once(once_attr, [&] {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES);
   });
   if (attr_err != cudaSuccess) return fail(FMOE_ERR_CUDA, "set-up of the e4m3 linear kernel failed: %s", cudaGetErrorString(attr_err));
   KernelParams p;
   p.token_tiles = (int)ceil_div<int64_t>(g.T, COLS);
   p.token_tile = (int)(ceil_div<int64_t>(ceil_div<int64_t>(g.T, p.token_tiles), 16) * 16);
   p.stage_bytes = HALVES * W_BYTES + p.token_tile * KBYTES;
-  p.stages = std::min(kMaxStages, (kMaxSmem - G::FIXED_BYTES) / p.stage_bytes);
+  p.stages = std::min(kMaxStages, (G::SMEM_BYTES - G::FIXED_BYTES) / p.stage_bytes);
   p.kblocks = (int)(g.k / 128);
   const int64_t row_tiles = ceil_div<int64_t>(g.n, 128);
-  const int sms = device_sm_count();
-  p.split = pick_split(row_tiles * p.token_tiles, p.kblocks, HALVES, p.token_tile, sms > 0 ? sms : 148);
+  p.split = split;
   const int64_t w_rows = HALVES * g.n;
   CUtensorMap map_x, map_w;
   int rc = pair_map_tokens(&map_x, g.x, g.T, g.k, 1, p.token_tile);
@@ -426,7 +485,7 @@ int launch(const LinearParams& g, cudaStream_t st) {
   p.n = g.n;
   p.activation = g.activation;
   p.early = g.behind_late_trigger;
-  launch_pdl_cluster(kernel, p.split, dim3((unsigned)(row_tiles * p.token_tiles * p.split)), dim3(G::THREADS), kMaxSmem, st, map_x, map_w, p);
+  launch_pdl_cluster(kernel, p.split, dim3((unsigned)(row_tiles * p.token_tiles * p.split)), dim3(G::THREADS), G::SMEM_BYTES, st, map_x, map_w, p);
   return launch_status("fp8_linear_kernel");
 }
 
@@ -434,8 +493,18 @@ int launch(const LinearParams& g, cudaStream_t st) {
 
 int run_linear(const LinearParams& p, bool gated, cudaStream_t st) {
   if (p.T <= 0) return FMOE_OK;
-  if (gated) return p.T <= 64 ? launch<2, 64>(p, st) : launch<2, 128>(p, st);
-  return p.T <= 64 ? launch<1, 64>(p, st) : launch<1, 128>(p, st);
+  const Choice c = choose(p, gated);
+  if (c.pair) return run_linear_pair(p, gated, c.split, st);
+  if (gated) {
+    if (p.T <= 16) return launch<Geo<2, 16, 4, 16, 1>>(p, c.split, st);
+    if (p.T <= 32) return launch<Geo<2, 32, 2, 32, 1>>(p, c.split, st);
+    if (p.T <= 64) return launch<Geo<2, 64, 1, 32, 1>>(p, c.split, st);
+    return launch<Geo<2, 128, 1, 64, 1>>(p, c.split, st);
+  }
+  if (p.T <= 16) return launch<Geo<1, 16, 4, 16, 2>>(p, c.split, st);
+  if (p.T <= 32) return launch<Geo<1, 32, 2, 32, 2>>(p, c.split, st);
+  if (p.T <= 64) return launch<Geo<1, 64, 1, 32, 1>>(p, c.split, st);
+  return launch<Geo<1, 128, 1, 32, 1>>(p, c.split, st);
 }
 
 namespace {
@@ -556,10 +625,17 @@ int64_t workspace_bytes(const fmoe_fp8_args* a, Call call, const char* who) {
 
 }  // namespace
 
+int status_word_linear_pair(int* out, bool clear);
+
+// of both kernels
 int status_word_linear(int* out, bool clear) {
   int zero = 0;
+  int pair = 0;
+  const int rc = status_word_linear_pair(&pair, clear);
+  if (rc) return rc;
   FMOE_CUDA_OK(cudaMemcpyFromSymbol(out, g_device_status_linear, sizeof(int)));
   if (clear && *out != 0) FMOE_CUDA_OK(cudaMemcpyToSymbol(g_device_status_linear, &zero, sizeof(int)));
+  if (*out == 0) *out = pair;
   return FMOE_OK;
 }
 

@@ -2,13 +2,24 @@
 //     h = round(x + r);  y = h / sqrt(mean(h^2) + eps) * w;  q = e4m3(y / s), s = max(amax(y), 1e-10) / 448 per 128 channels
 //     (or one s per row), norm = round(y)
 // A CTA owns a row at a time and keeps it in registers between the sum of squares and the outputs, so every byte is read and
-// written once: HBM bounds it from a few MB on, the launch and two dependent reductions below that.
+// written once: HBM bounds it from some ten MB on (beside the issue slots, where a row has neither residual nor norm to move), the
+// launch and the dependent reductions below that: one row of 7168 takes 3 us.
 #include <algorithm>
+#include <type_traits>
 
+#include "ptx_sm100.cuh"
 #include "rows.cuh"
 
 namespace fmoe {
+
+// This translation unit's status word; read by status_word_norm().
+__device__ int g_device_status_norm = 0;
+
 namespace {
+
+constexpr int kMaxStages = 4;
+constexpr int kStreamBytes = 220 * 1024;  // shared memory of an SM for the rows on their way
+__device__ __forceinline__ void report(int code) { atomicCAS(&g_device_status_norm, 0, code); }
 
 struct NormParams {
   const void* x;
@@ -20,7 +31,7 @@ struct NormParams {
   int64_t x_stride, residual_stride, rows;
   int K;
   int weight_f32;
-  float eps;
+  float eps, inv_K;
 };
 
 // eight consecutive values
@@ -47,9 +58,32 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
+// Division costs most instructions of this kernel where it is written as __fdiv_rn (42 per value in all, issue slots 74 % busy: 8192 rows of
+// 7168 in 93 us).  Here a quotient is a product with the reciprocal and one correction by its exact remainder, whose error is far below
+// half a unit in the last place; for the scale, whose divisor is a constant, that is the correctly rounded quotient for every significand
+// (all 2^23 compared), so that scales are the quantiser's bits.
+__device__ __forceinline__ float corrected(float v, float d, float r) {
+  const float q = v * r;
+  return fmaf(fmaf(-q, d, v), r, q);
+}
+__device__ __forceinline__ float scale_448(float amax) {
+  return amax <= 3.0e38f ? corrected(amax, 448.0f, 1.0f / 448.0f) : __fdiv_rn(amax, 448.0f);
+}
+// eight values over s -> e4m3
+__device__ __forceinline__ uint2 quant8_corrected(const float (&v)[8], float s, bool finite) {
+  if (!finite) return quant8(v, s, 0.f, false);
+  const float r = __fdividef(1.0f, s);
+  uint32_t half[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    half[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(corrected(v[2 * i], s, r), corrected(v[2 * i + 1], s, r)), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(half[0] | half[1] << 16, half[2] | half[3] << 16);
+}
+
 // Reduction over the CTA's warps, the same value in every thread.  `buf` holds a value per warp; two calls in a row use two.
+// False, to every thread, if any thread's `fine` is.
 template <bool MAX>
-__device__ __forceinline__ float cta_reduce(float v, float* buf) {
+__device__ __forceinline__ bool cta_reduce(float& v, float* buf, bool fine) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     const float o = __shfl_xor_sync(0xffffffffu, v, off);
@@ -57,16 +91,86 @@ __device__ __forceinline__ float cta_reduce(float v, float* buf) {
   }
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   if (lane == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
+  fine = __syncthreads_and(fine);
   v = lane < warps ? buf[lane] : 0.f;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     const float o = __shfl_xor_sync(0xffffffffu, v, off);
     v = MAX ? fmaxf(v, o) : v + o;
   }
-  return v;
+  return fine;
 }
 
+// The rest of a row whose sums h are in registers: sum of squares, norm, scales, e4m3.  `fine` (of this thread) is false where
+// its loads did not arrive; false is returned to every thread then, and nothing of the row has been written here.
+template <typename T, int VECS, bool PER_TOKEN>
+__device__ __forceinline__ bool finish_row(const NormParams& p, int64_t row, float (&h)[VECS][8], float (*buf)[32], bool fine) {
+  const int vecs = p.K / 8;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
+  }
+  if (!cta_reduce<false>(sum, buf[0], fine)) return false;
+  const float rstd = rsqrtf(fmaf(sum, p.inv_K, p.eps));
+  float amax_row = 0.f;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c < vecs) {
+      float w[8];
+      if (p.weight_f32) load8(reinterpret_cast<const float*>(p.weight) + 8 * c, w);
+      else load8(reinterpret_cast<const __nv_bfloat16*>(p.weight) + 8 * c, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        h[i][j] = h[i][j] * rstd * w[j];
+        if (PER_TOKEN) amax_row = fmaxf(amax_row, fabsf(h[i][j]));
+      }
+      if (p.norm) store8(reinterpret_cast<T*>(p.norm) + row * p.K + 8 * c, h[i]);
+    }
+  }
+  float s_row = 0.f;
+  if constexpr (PER_TOKEN) {
+    cta_reduce<true>(amax_row, buf[1], true);
+    s_row = fmaxf(scale_448(amax_row), 1.0f / (448.0f * 512.0f));
+    if (threadIdx.x == 0) p.scale[row] = s_row;
+  }
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    float amax = amax_row, s = s_row;
+    if constexpr (!PER_TOKEN) {  // a group is the vectors of 16 neighbouring lanes: K is a multiple of 128
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(h[i][j]));
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+      s = scale_448(fmaxf(amax, 1e-10f));
+    }
+    if (c < vecs) {
+      *reinterpret_cast<uint2*>(p.q + row * p.K + 8 * c) = quant8_corrected(h[i], s, amax <= 3.0e38f);
+      if (!PER_TOKEN && c % 16 == 0) p.scale[row * (p.K / 128) + c / 16] = s;
+    }
+  }
+  if constexpr (!PER_TOKEN) __syncthreads();  // the warps' sums have been read by everyone (PER_TOKEN: cta_reduce's barrier)
+  return true;
+}
+
+// h = x, or round(x + r) which is stored
+template <typename T, int VECS>
+__device__ __forceinline__ void add_residual(const NormParams& p, T* res, float (&h)[VECS][8], const float (&r)[VECS][8]) {
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (8 * c < p.K) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[i][j] = to_f32(from_f32<T>(h[i][j] + r[i][j]));
+      store8(res + 8 * c, h[i]);
+    }
+  }
+}
+
+// Few rows: a CTA per row, loads straight into registers.
 template <typename T, int VECS, bool PER_TOKEN>
 __global__ void __launch_bounds__(1024)
 rms_norm_quant_kernel(const NormParams p) {
@@ -76,8 +180,68 @@ rms_norm_quant_kernel(const NormParams p) {
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
     T* res = p.residual ? reinterpret_cast<T*>(p.residual) + row * p.residual_stride : nullptr;
+    float h[VECS][8], r[VECS][8];
+    // every load of the row is on its way before the first sum is stored
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
+      if (c < vecs) {
+        load8(x + 8 * c, h[i]);
+        if (res) load8(res + 8 * c, r[i]);
+      }
+    }
+    if (res) add_residual<T, VECS>(p, res, h, r);
+    finish_row<T, VECS, PER_TOKEN>(p, row, h, buf, true);
+  }
+}
+
+// Many bf16 rows: persistent CTAs whose rows arrive in a ring of shared memory (one bulk copy per row and tensor), so that the next
+// rows' bytes are on their way while this one is reduced.  8192 rows of 7168 with residual and norm: 135 us with loads into registers
+// (two CTAs of 448 threads fit an SM, 57 KB on their way), 90 us here, 5.9 TB/s.  Rows of fp32 have twice the bytes per thread and do
+// better without the detour: 4096 rows of 8192 90 us (5.8 TB/s) against 104.  Four 16-byte pieces per thread instead of two spread the
+// reductions over more values but leave fewer warps: 93 us.
+template <bool PER_TOKEN, int MAX_THREADS>
+__global__ void __launch_bounds__(MAX_THREADS, MAX_THREADS > 512 ? 1 : 3)
+rms_norm_quant_stream_kernel(const NormParams p, int stages) {
+  using T = __nv_bfloat16;
+  constexpr int VECS = 2;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float buf[2][32];
+  __shared__ uint64_t full[kMaxStages];
+  const int vecs = p.K / 8, row_bytes = p.K * (int)sizeof(T), stage_bytes = row_bytes * (p.residual ? 2 : 1);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) ptx::mbar_init(&full[s], 1);
+    ptx::fence_barrier_init();
+  }
+  __syncthreads();
+  pdl_entry_late();
+  auto fetch = [&](int64_t row, int s) {
+    ptx::mbar_arrive_expect_tx(&full[s], stage_bytes);
+    ptx::bulk_load(ptx::smem_u32(ring + s * stage_bytes), reinterpret_cast<const T*>(p.x) + row * p.x_stride, row_bytes, ptx::smem_u32(&full[s]));
+    if (p.residual)
+      ptx::bulk_load(ptx::smem_u32(ring + s * stage_bytes + row_bytes), reinterpret_cast<const T*>(p.residual) + row * p.residual_stride, row_bytes,
+                     ptx::smem_u32(&full[s]));
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s)
+      if (blockIdx.x + (int64_t)s * gridDim.x < p.rows) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+  }
+  int stage = 0;
+  uint32_t phase = 0;
+  int64_t next = blockIdx.x + (int64_t)stages * gridDim.x;
+  bool alive = true;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, next += gridDim.x) {
+    T* res = p.residual ? reinterpret_cast<T*>(p.residual) + row * p.residual_stride : nullptr;
+    const T* x = reinterpret_cast<const T*>(ring + stage * stage_bytes);
     float h[VECS][8];
-    float sum = 0.f;
+    bool fine = ptx::mbar_wait(&full[stage], phase);
+    // all threads agree before the first store, and again in the sum of squares, which all of them have read the stage for
+    if (res && !__syncthreads_and(fine)) {
+      alive = false;
+      break;
+    }
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
@@ -87,60 +251,33 @@ rms_norm_quant_kernel(const NormParams p) {
         load8(x + 8 * c, h[i]);
         if (res) {
           float r[8];
-          load8(res + 8 * c, r);
+          load8(reinterpret_cast<const T*>(ring + stage * stage_bytes + row_bytes) + 8 * c, r);
 #pragma unroll
           for (int j = 0; j < 8; ++j) h[i][j] = to_f32(from_f32<T>(h[i][j] + r[j]));
           store8(res + 8 * c, h[i]);
         }
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
     }
-    sum = cta_reduce<false>(sum, buf[0]);
-    const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(sum, (float)p.K) + p.eps));
-    float amax_row = 0.f;
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      if (c < vecs) {
-        float w[8];
-        if (p.weight_f32) load8(reinterpret_cast<const float*>(p.weight) + 8 * c, w);
-        else load8(reinterpret_cast<const __nv_bfloat16*>(p.weight) + 8 * c, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          h[i][j] = h[i][j] * rstd * w[j];
-          if (PER_TOKEN) amax_row = fmaxf(amax_row, fabsf(h[i][j]));
-        }
-        if (p.norm) store8(reinterpret_cast<T*>(p.norm) + row * p.K + 8 * c, h[i]);
-      }
+    if (!finish_row<T, VECS, PER_TOKEN>(p, row, h, buf, fine)) {
+      alive = false;
+      break;
     }
-    float s_row = 0.f;
-    if constexpr (PER_TOKEN) {
-      amax_row = cta_reduce<true>(amax_row, buf[1]);
-      s_row = fmaxf(__fdiv_rn(amax_row, 448.0f), 1.0f / (448.0f * 512.0f));
-      if (threadIdx.x == 0) p.scale[row] = s_row;
+    if (threadIdx.x == 0 && next < p.rows) fetch(next, stage);
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
     }
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      float amax = amax_row, s = s_row;
-      if constexpr (!PER_TOKEN) {  // a group is the vectors of 16 neighbouring lanes: K is a multiple of 128
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(h[i][j]));
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-        s = group_scale(amax);
-      }
-      if (c < vecs) {
-        *reinterpret_cast<uint2*>(p.q + row * p.K + 8 * c) = quant8(h[i], s, __frcp_rn(s), amax <= 3.0e38f);
-        if (!PER_TOKEN && c % 16 == 0) p.scale[row * (p.K / 128) + c / 16] = s;
-      }
-    }
-    if constexpr (!PER_TOKEN) __syncthreads();  // the sums of this row have been read by everyone (PER_TOKEN: cta_reduce's barrier)
+  }
+  if (!alive && threadIdx.x == 0) {
+    report(0x3100);
+    for (int s = 0; s < stages; ++s) ptx::mbar_wait(&full[s], s < stage ? phase ^ 1 : phase);  // copies still on their way
   }
 }
 
 }  // namespace
+
+int status_word_norm(int* out, bool clear);
+
 }  // namespace fmoe
 
 extern "C" int fmoe_rms_norm_quant(const void* x, int64_t x_stride, void* residual, int64_t residual_stride, int dtype, const void* weight,
@@ -161,17 +298,52 @@ extern "C" int fmoe_rms_norm_quant(const void* x, int64_t x_stride, void* residu
   FMOE_REQUIRE(aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(norm) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0 &&
                    (reinterpret_cast<uintptr_t>(scale) & 3u) == 0,
                "rms_norm_quant: misaligned pointer");
-  NormParams p{x, residual, weight, (uint8_t*)q, scale, norm, x_stride, residual_stride, rows, (int)K, weight_dtype == FMOE_F32, eps};
+  NormParams p{x, residual, weight, (uint8_t*)q, scale, norm, x_stride, residual_stride, rows, (int)K, weight_dtype == FMOE_F32, eps, 1.0f / (float)K};
   const int vecs = (int)(K / 8);
-  auto go = [&](auto vecs_c) {
-    constexpr int V = decltype(vecs_c)::value;
-    const unsigned threads = (unsigned)(ceil_div(ceil_div(vecs, V), 32) * 32);
-    const unsigned grid = (unsigned)std::min<int64_t>(rows, 148 * 32);
-    auto with = [&](auto kernel) { launch_pdl(kernel, dim3(grid), dim3(threads), 0, (cudaStream_t)stream, p); };
-    if (dtype == FMOE_BF16) per_token ? with(rms_norm_quant_kernel<__nv_bfloat16, V, true>) : with(rms_norm_quant_kernel<__nv_bfloat16, V, false>);
-    else per_token ? with(rms_norm_quant_kernel<float, V, true>) : with(rms_norm_quant_kernel<float, V, false>);
+  const auto st = (cudaStream_t)stream;
+  auto threads = [&](int v) { return (unsigned)(ceil_div(ceil_div(vecs, v), 32) * 32); };
+  auto each_type = [&](auto go) {  // go(type, per_token)
+    if (dtype == FMOE_BF16) per_token ? go((__nv_bfloat16*)nullptr, std::true_type{}) : go((__nv_bfloat16*)nullptr, std::false_type{});
+    else per_token ? go((float*)nullptr, std::true_type{}) : go((float*)nullptr, std::false_type{});
   };
-  if (vecs <= 1024) go(std::integral_constant<int, 1>{});
-  else go(std::integral_constant<int, 2>{});
+  if (dtype == FMOE_BF16 && rows > 296) {  // 400 rows of 7168: 6.3 us, in registers 7.9; 77 rows 3.9 and 3.7
+    const int stage_bytes = (int)K * 2 * (residual ? 2 : 1);
+    const int ctas = std::min(std::max(1, 1536 / (int)threads(2)), (kStreamBytes - 2048) / (2 * stage_bytes + 1024));  // at least 1: K <= 16384
+    const int stages = std::min(kMaxStages, (kStreamBytes / ctas - 1024) / stage_bytes);
+    cudaError_t attr_err = cudaSuccess;
+    auto go = [&](auto token) {
+      constexpr bool PER_TOKEN = decltype(token)::value;
+      auto kernel = rms_norm_quant_stream_kernel<PER_TOKEN, 512>;
+      auto wide = rms_norm_quant_stream_kernel<PER_TOKEN, 1024>;
+      static PerDeviceOnce once_attr;
+      attr_err = per_device_once(once_attr, [&] {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(wide, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
+      });
+      if (attr_err != cudaSuccess) return;
+      const unsigned grid = (unsigned)std::min<int64_t>(rows, (int64_t)148 * ctas);
+      launch_pdl(threads(2) > 512 ? wide : kernel, dim3(grid), dim3(threads(2)), (size_t)stages * stage_bytes, st, p, stages);
+    };
+    if (per_token) go(std::true_type{});
+    else go(std::false_type{});
+    if (attr_err != cudaSuccess) return fail(FMOE_ERR_CUDA, "set-up of the norm kernel failed: %s", cudaGetErrorString(attr_err));
+    return launch_status("rms_norm_quant_stream_kernel");
+  }
+  each_type([&](auto* type, auto token) {
+    using E = std::remove_pointer_t<decltype(type)>;
+    auto with = [&](auto v) {
+      constexpr int VV = decltype(v)::value;
+      launch_pdl(rms_norm_quant_kernel<E, VV, decltype(token)::value>, dim3((unsigned)std::min<int64_t>(rows, 148 * 32)), dim3(threads(VV)), 0, st, p);
+    };
+    if (vecs <= 1024 && rows <= 296) with(std::integral_constant<int, 1>{});
+    else with(std::integral_constant<int, 2>{});
+  });
   return launch_status("rms_norm_quant_kernel");
+}
+
+int fmoe::status_word_norm(int* out, bool clear) {
+  int zero = 0;
+  FMOE_CUDA_OK(cudaMemcpyFromSymbol(out, fmoe::g_device_status_norm, sizeof(int)));
+  if (clear && *out != 0) FMOE_CUDA_OK(cudaMemcpyToSymbol(fmoe::g_device_status_norm, &zero, sizeof(int)));
+  return FMOE_OK;
 }

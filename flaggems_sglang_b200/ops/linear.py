@@ -8,59 +8,67 @@ from .. import _C
 _ACTIVATIONS = ("silu", "gelu")
 
 
+# A call on a few tokens lasts as long as these functions: attributes are read once, and tensors as they usually come (contiguous, 16-byte
+# aligned) are taken as they are.
 def _input(x: torch.Tensor, x_scale: torch.Tensor | None):
-    """-> (rows, their scales or None, type code): bf16 rows that the call quantises, or e4m3 rows with a scale per 128 channels."""
+    """-> (rows, their scales or None, T, K, type code): bf16 rows that the call quantises, or e4m3 rows with a scale per 128 channels."""
     if x.dim() != 2:
         raise ValueError("x must be a 2-D tensor")
     T, K = x.shape
     if K == 0 or K % 128:
         raise ValueError(f"rows of {K} channels: a multiple of 128 is needed")
-    if x.dtype == torch.float8_e4m3fn:
-        if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (T, K // 128):
+    if x.dtype is torch.float8_e4m3fn:
+        if x_scale is None or x_scale.dtype is not torch.float32 or x_scale.shape != (T, K // 128):
             raise ValueError("e4m3 x needs x_scale, fp32 [rows, K/128]")
-        return _aligned(x), x_scale.contiguous(), _C.E4M3
-    if x.dtype != torch.bfloat16:
+        return _aligned(x), x_scale if x_scale.is_contiguous() else x_scale.contiguous(), T, K, _C.E4M3
+    if x.dtype is not torch.bfloat16:
         raise ValueError("x must be bf16 or e4m3")
     if x_scale is not None:
         raise ValueError("x_scale belongs to e4m3 x")
-    return _aligned(x), None, _C.BF16
+    return _aligned(x), None, T, K, _C.BF16
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _weight(w: torch.Tensor, scale: torch.Tensor, K: int, name: str):
-    if w.dim() != 2 or w.dtype != torch.float8_e4m3fn or w.shape[1] != K or w.shape[0] == 0:
+    """-> (weights, scales, N)"""
+    if w.dim() != 2 or w.dtype is not torch.float8_e4m3fn:
         raise ValueError(f"{name} must be e4m3 [N, {K}]")
-    if scale.dtype != torch.float32 or tuple(scale.shape) != ((w.shape[0] + 127) // 128, K // 128):
+    N, k = w.shape
+    if k != K or N == 0:
+        raise ValueError(f"{name} must be e4m3 [N, {K}]")
+    if scale.dtype is not torch.float32 or scale.shape != ((N + 127) // 128, K // 128):
         raise ValueError(f"the scales of {name} must be fp32 [ceil(N/128), {K // 128}]")
-    return _aligned(w), scale.contiguous()
+    return _aligned(w), scale if scale.is_contiguous() else scale.contiguous(), N
 
 
-def _extras(bias, addend, T: int, N: int):
-    if bias is not None:
-        if tuple(bias.shape) != (N,) or bias.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError("bias must be fp32 or bf16 [N]")
-        bias = _aligned(bias.float())
-    if addend is not None:
-        if tuple(addend.shape) != (T, N) or addend.dtype != torch.bfloat16:
-            raise ValueError("addend must be bf16 [rows, N]")
-        addend = _aligned(addend)
-    return bias, addend
+def _bias(bias: torch.Tensor, N: int) -> torch.Tensor:
+    if bias.shape != (N,) or bias.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("bias must be fp32 or bf16 [N]")
+    return _aligned(bias.float())
 
 
-def _call(name: str, args: _C.Fp8Args, dev: torch.device) -> None:
-    lib = _C.lib()
-    need = getattr(lib, name + "_workspace_bytes")(args)
-    if need < 0:
-        _C.check(_C.ERR_INVALID_ARG)
-    ws = None
+def _addend(addend: torch.Tensor, T: int, N: int) -> torch.Tensor:
+    if addend.shape != (T, N) or addend.dtype is not torch.bfloat16:
+        raise ValueError("addend must be bf16 [rows, N]")
+    return _aligned(addend)
+
+
+def _call(run, workspace_bytes, args: _C.Fp8Args, dev: torch.device) -> None:
+    if dev.index != _C.current_device():
+        with _C.on_device(dev):
+            return _call(run, workspace_bytes, args, dev)
+    need = workspace_bytes(args)
     if need:
-        ws = torch.empty(int(need), dtype=torch.uint8, device=dev)
+        if need < 0:
+            _C.check(_C.ERR_INVALID_ARG)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _C.check(getattr(lib, name)(args, _C.stream_ptr(dev)))
+    _C.check(run(args, _C.stream_ptr(dev)))
 
 
 def fp8_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale: torch.Tensor | None = None,
@@ -72,18 +80,18 @@ def fp8_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_
     residual, another branch's output) join them before the one rounding.  K is a multiple of 128, N of 8.
     """
     dev = _C.require_cuda(x, w, w_scale, x_scale, bias, addend)
-    x, x_scale, code = _input(x, x_scale)
-    T, K = x.shape
-    w, w_scale = _weight(w, w_scale, K, "w")
-    N = w.shape[0]
+    x, x_scale, T, K, code = _input(x, x_scale)
+    w, w_scale, N = _weight(w, w_scale, K, "w")
     if N % 8:
         raise ValueError(f"w has {N} rows: a multiple of 8 is needed")
-    bias, addend = _extras(bias, addend, T, N)
+    if bias is not None:
+        bias = _bias(bias, N)
+    if addend is not None:
+        addend = _addend(addend, T, N)
     out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
-    if T == 0:
-        return out
-    with _C.on_device(dev):
-        _call("fmoe_fp8_linear", _C.Fp8Args(
+    if T:
+        lib = _C.lib()
+        _call(lib.fmoe_fp8_linear, lib.fmoe_fp8_linear_workspace_bytes, _C.Fp8Args(
             x_dtype=code, T=T, K=K, N=N, x=x.data_ptr(), x_scale=_C.ptr(x_scale), w=w.data_ptr(), w_scale=w_scale.data_ptr(),
             bias=_C.ptr(bias), addend=_C.ptr(addend), out=out.data_ptr()), dev)
     return out
@@ -101,22 +109,20 @@ def fp8_gated_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w
     dev = _C.require_cuda(x, w13, w13_scale, w2, w2_scale, x_scale, addend)
     if activation not in _ACTIVATIONS:
         raise ValueError(f"Unsupported activation: {activation}")
-    x, x_scale, code = _input(x, x_scale)
-    T, K = x.shape
-    w13, w13_scale = _weight(w13, w13_scale, K, "w13")
-    if w13.shape[0] % 256:
-        raise ValueError(f"w13 has {w13.shape[0]} rows: 2I with I a multiple of 128 is needed")
-    I = w13.shape[0] // 2
-    w2, w2_scale = _weight(w2, w2_scale, I, "w2")
-    N = w2.shape[0]
+    x, x_scale, T, K, code = _input(x, x_scale)
+    w13, w13_scale, rows = _weight(w13, w13_scale, K, "w13")
+    if rows % 256:
+        raise ValueError(f"w13 has {rows} rows: 2I with I a multiple of 128 is needed")
+    I = rows // 2
+    w2, w2_scale, N = _weight(w2, w2_scale, I, "w2")
     if N % 8:
         raise ValueError(f"w2 has {N} rows: a multiple of 8 is needed")
-    _, addend = _extras(None, addend, T, N)
+    if addend is not None:
+        addend = _addend(addend, T, N)
     out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
-    if T == 0:
-        return out
-    with _C.on_device(dev):
-        _call("fmoe_fp8_mlp", _C.Fp8Args(
+    if T:
+        lib = _C.lib()
+        _call(lib.fmoe_fp8_mlp, lib.fmoe_fp8_mlp_workspace_bytes, _C.Fp8Args(
             x_dtype=code, activation=_C.ACTIVATIONS[activation], T=T, K=K, N=N, I=I, x=x.data_ptr(), x_scale=_C.ptr(x_scale),
             w=w13.data_ptr(), w_scale=w13_scale.data_ptr(), w2=w2.data_ptr(), w2_scale=w2_scale.data_ptr(),
             addend=_C.ptr(addend), out=out.data_ptr()), dev)

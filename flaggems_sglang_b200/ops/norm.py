@@ -6,6 +6,9 @@ import torch
 from .. import _C
 
 
+_CODES = {torch.bfloat16: _C.BF16, torch.float32: _C.F32}
+
+
 def _rows(t: torch.Tensor) -> bool:
     """Rows that the kernel reads in place: contiguous channels, rows at multiples of 16 bytes that do not overlap."""
     per16 = 16 // t.element_size()
@@ -23,35 +26,47 @@ def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     y in x's type, for what reads the layer's input unquantised (a router, bf16 experts).
     K is a multiple of 128 (``per_token``: of 8), at most 16384.  Rows of x and residual may be strided; weight is bf16 or fp32 [K].
     """
+    # a call on a few rows lasts as long as this function: attributes are read once, the common layout is taken as it is
     dev = _C.require_cuda(x, weight, residual)
-    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
+    code, w_code = _CODES.get(x.dtype), _CODES.get(weight.dtype)
+    if x.dim() != 2 or code is None:
         raise ValueError("x must be a 2-D bf16 or fp32 tensor")
     rows, K = x.shape
-    if weight.shape != (K,) or weight.dtype not in (torch.bfloat16, torch.float32):
+    if weight.dim() != 1 or weight.numel() != K or w_code is None:
         raise ValueError("weight must be a bf16 or fp32 tensor of x's row length")
     if K == 0 or K > 16384 or K % (8 if per_token else 128):
         raise ValueError(f"rows of {K} channels: a multiple of {8 if per_token else 128} up to 16384 is needed")
-    if not _rows(x):
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-    weight = weight.contiguous()
-    if weight.data_ptr() % 16:
-        weight = weight.clone()
+    x_ptr, x_stride = x.data_ptr(), K
+    dense = x.is_contiguous() and x_ptr % 16 == 0
+    if not dense:
+        if not _rows(x):
+            x = x.contiguous() if not x.is_contiguous() else x.clone()
+        x_ptr, x_stride = x.data_ptr(), x.stride(0) if rows > 1 else K
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    r_ptr, r_stride = None, K
     if residual is not None:
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError("residual must have x's shape and type")
-        if not _rows(residual):
-            raise ValueError("residual is updated in place: its channels must be contiguous and its rows start at multiples of 16 bytes")
-    q = torch.empty(rows, K, dtype=torch.float8_e4m3fn, device=dev)
-    s = torch.empty((rows,) if per_token else (rows, K // 128), dtype=torch.float32, device=dev)
-    norm = torch.empty(rows, K, dtype=x.dtype, device=dev) if return_norm else None
-    with _C.on_device(dev):
-        _C.check(_C.lib().fmoe_rms_norm_quant(
-            x.data_ptr(), x.stride(0) if rows > 1 else K, _C.ptr(residual),
-            (residual.stride(0) if rows > 1 else K) if residual is not None else K,
-            _C.DTYPE_CODE[x.dtype], weight.data_ptr(), _C.DTYPE_CODE[weight.dtype], rows, K, eps, int(per_token), q.data_ptr(),
-            s.data_ptr(), _C.ptr(norm), _C.stream_ptr(dev)))
+        r_ptr = residual.data_ptr()
+        if not (residual.is_contiguous() and r_ptr % 16 == 0):
+            if not _rows(residual):
+                raise ValueError("residual is updated in place: its channels must be contiguous and its rows start at multiples of 16 bytes")
+            r_stride = residual.stride(0) if rows > 1 else K
+    if dense:
+        q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+        norm = torch.empty_like(x) if return_norm else None
+    else:
+        q = torch.empty(rows, K, dtype=torch.float8_e4m3fn, device=dev)
+        norm = torch.empty(rows, K, dtype=x.dtype, device=dev) if return_norm else None
+    s = torch.empty(rows, dtype=torch.float32, device=dev) if per_token else torch.empty(rows, K // 128, dtype=torch.float32, device=dev)
+    args = (x_ptr, x_stride, r_ptr, r_stride, code, weight.data_ptr(), w_code, rows, K, eps, int(per_token), q.data_ptr(), s.data_ptr(),
+            None if norm is None else norm.data_ptr(), _C.stream_ptr(dev))
+    if dev.index == _C.current_device():
+        _C.check(_C.lib().fmoe_rms_norm_quant(*args))
+    else:
+        with _C.on_device(dev):
+            _C.check(_C.lib().fmoe_rms_norm_quant(*args))
     return (q, s, norm) if return_norm else (q, s)
 
 
