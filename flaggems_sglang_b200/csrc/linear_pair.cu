@@ -1,19 +1,21 @@
 // Dense e4m3 products with block scales for many tokens (linear.cuh): persistent CTA pairs (cta_group::2).
 //
-//   tile      : 256 tokens on M (128 in each CTA) x 256 weight rows on N (128 loaded by each CTA; gate/up: 64 gate rows and the
-//               same 64 up rows of the tile's 128 channels).  A thread of the fold owns one token: its activation scale is one
+//   tile      : 256 tokens on M (128 in each CTA) x 256 weight rows on N in two halves: 128 channels each, or (gate/up) 64 gate rows and
+//               the same 64 up rows; a CTA loads 64 rows of either.  A thread of the fold owns one token: its activation scale is one
 //               value per K block, and the weight scale one value per 128 rows
-//   K block   : 128 bytes per row; 4 MMAs of 256 x 256 x 32 into a fresh TMEM partial of 256 columns, of which there are two
-//   warps 0-7 : fold + epilogue.  Warp w: TMEM lanes 32 * (w % 4).., the 128 columns of CTA w / 4's weight rows: 128 sums per thread,
-//               and 64 further registers for the columns on their way: while 32 are added the next 32 are being read, and the
-//               partial is handed back before the last 32 are added
+//   K block   : 128 bytes per row; for each half 4 MMAs of 256 x 128 x 32 into a fresh TMEM partial of 128 columns, of which there are four
+//   warps 0-7 : fold + epilogue.  Warp w: TMEM lanes 32 * (w % 4).., half w / 4: 128 sums per thread, and 64 further registers for the
+//               columns on their way: each 32 are replaced by the next as soon as they have been added, and the partial is handed back
+//               before the last 64 are.  The two halves' warps run half a K block apart, so that one's reads and waits are beside the
+//               other's FMAs
 //   warps 8, 9: TMA (tokens, weights)     warp 10: MMA (CTA 0)     warp 11: scales, eight K blocks at a time, transposed into a ring
 // SPLIT: up to four pairs of a cluster share a tile's K blocks; their sums meet through distributed shared memory as in linear.cu.
-// One MMA over all 256 rows of N, because shared memory is what a pair runs out of first: 32 KB in and 32 KB of operand reads per K
-// block are 512 of its clocks, as many as the MMAs take; two MMAs of 128 rows read the tokens twice (48 KB, 640 clocks).
-// What bounds it: 820 clocks per K block and tile, the fold's chain of waits, TMEM reads and FMAs (without the FMAs 730; with nothing
-// folded at all 655, which is what an SM takes in from L2), and the power limit from some 2000 tokens on (8192 x 7168 x 4096: 217 us,
-// 2.2 PFLOP/s at about 1.5 GHz).  An arrival behind a branch left the fold's warps split, so that each FMA was issued twice: 247 us.
+// What bounds it: up to some 1500 tokens about 800 clocks per K block and tile, of which shared memory (32 KB in, 48 KB of operands at 128
+// bytes per clock) needs 640 and what an SM takes in from L2 655; from there on the power limit (8192 x 7168 x 4096: 210 us, 2.3 PFLOP/s
+// at about 1.5 GHz).  Tried: one MMA over all 256 rows of N (512 clocks of shared memory, but only two partials for the fold's round
+// trip: the same at 8192 tokens, 2048 x 2048 x 7168 42 us against 38); reads of the next K block before the last of this one are added
+// (30.5 us against 28.4 for one round of K = 7168).  An arrival behind a branch left the fold's warps split, so that each FMA was issued
+// twice: 247 us at 8192 tokens where it now takes 217 with the same epilogue.
 #include "linear.cuh"
 #include "pair.cuh"
 #include "rows.cuh"
@@ -37,13 +39,15 @@ constexpr int kFoldWarps = 8;
 constexpr int kThreads = (kFoldWarps + 4) * 32;
 constexpr int kFoldRegs = 216, kOtherRegs = 72;   // together the launch's 384 x 168
 constexpr int kGroup = 8;                         // K blocks per slot of scales
-constexpr int kSlots = 4;
+constexpr int kSlots = 3;
 constexpr int SLOT_FLOATS = kGroup * (128 + 2);   // [K block][token], [K block][weight block]
 constexpr int BAR_BYTES = 512;
 constexpr int SUM_PITCH = 260;                    // floats from token to token: 16-byte accesses of eight lanes take all banks
 constexpr int kMaxSplit = kMaxPairSplit;
 constexpr int AMAX_FLOATS = 2 * 2 * 128;          // [tile parity][column half][token]
-constexpr int kSmemBytes = STAGES * STAGE_BYTES + BAR_BYTES + (kSlots * SLOT_FLOATS + AMAX_FLOATS) * 4;
+constexpr int STRIP_PITCH = 80;                    // bytes from token to token of a fold warp's strip: 64 and a shift of banks
+constexpr int STRIP_BYTES = 32 * STRIP_PITCH;
+constexpr int kSmemBytes = STAGES * STAGE_BYTES + BAR_BYTES + (kSlots * SLOT_FLOATS + AMAX_FLOATS) * 4 + kFoldWarps * STRIP_BYTES;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 
 struct KernelParams {
@@ -91,14 +95,15 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
   uint64_t* full_bar = bars;                // [STAGES] used in CTA 0: both CTAs' loads -> MMA
   uint64_t* empty_bar = bars + STAGES;      // [STAGES] per CTA: MMA -> TMA
-  uint64_t* part_full = bars + 2 * STAGES;  // [2] per CTA: MMA -> fold
-  uint64_t* part_empty = part_full + 2;     // [2] used in CTA 0: folds of both CTAs -> MMA
-  uint64_t* sc_full = part_empty + 2;       // [kSlots]
+  uint64_t* part_full = bars + 2 * STAGES;  // [4] per CTA: MMA -> fold; 2 * (K block % 2) + half
+  uint64_t* part_empty = part_full + 4;     // [4] used in CTA 0: folds of both CTAs -> MMA
+  uint64_t* sc_full = part_empty + 4;       // [kSlots]
   uint64_t* sc_empty = sc_full + kSlots;    // [kSlots]
   uint64_t* amax_bar = sc_empty + kSlots;   // [4] the two warps that hold a token's 128 channels
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(amax_bar + 4);
   float* scales = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES + BAR_BYTES);
   float* amax_buf = scales + kSlots * SLOT_FLOATS;
+  uint8_t* strips = reinterpret_cast<uint8_t*>(amax_buf + AMAX_FLOATS);
 
   const int warp = ptx::uniform_warp_id(), lane = threadIdx.x & 31;
   const int cluster_rank = (int)ptx::cluster_ctarank(), rank = cluster_rank & 1;
@@ -112,9 +117,9 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       ptx::mbar_init(&full_bar[s], 1);
       ptx::mbar_init(&empty_bar[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 4; ++b) {
       ptx::mbar_init(&part_full[b], 1);
-      ptx::mbar_init(&part_empty[b], 2 * kFoldWarps);
+      ptx::mbar_init(&part_empty[b], kFoldWarps);  // the half's four warps of both CTAs
     }
     for (int s = 0; s < kSlots; ++s) {
       ptx::mbar_init(&sc_full[s], 1);
@@ -143,7 +148,7 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     if constexpr (MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFoldRegs));
     pdl_entry_late();
     const int quarter = warp & 3, piece = warp >> 2;
-    const uint32_t from = tmem_base + ((uint32_t)(quarter * 32) << 16) + 128 * piece;
+    const uint32_t from = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t empty0 = ptx::smem_u32(part_empty) & ~ptx::kPeerRankBit;
     uint32_t step = 0, sc_step = 0;  // K blocks folded so far; the same with whole slots of scales for every tile
     bool alive = true;
@@ -166,7 +171,7 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         const float a = sc[(sc_step % kGroup) * 128 + quarter * 32 + lane];
         const float2 w = *reinterpret_cast<const float2*>(sc + kGroup * 128 + (sc_step % kGroup) * 2);
         const float f0 = a * (GATED ? w.x : (piece ? w.y : w.x)), f1 = GATED ? a * w.y : f0;
-        const uint32_t buf = step & 1;
+        const uint32_t buf = 2 * (step & 1) + piece;
         if (!warp_wait(&part_full[buf], (step >> 1) & 1)) {
           report(0x2440);
           alive = false;
@@ -175,7 +180,7 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         ptx::tc_fence_after_sync();
         // two reads of 32 columns are in flight; each is replaced by the next as soon as it has been added
         uint32_t v[2][32];
-        const uint32_t at = from + buf * 256;
+        const uint32_t at = from + buf * 128;
         auto add = [&](auto c_c) {
           constexpr int c = decltype(c_c)::value;
 #pragma unroll
@@ -212,7 +217,15 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         sc_step += kGroup - sc_step % kGroup;
       }
 
-      const int64_t t = (int64_t)tl.token * 256 + rank * 128 + quarter * 32 + lane;
+      // The warp's 32 tokens leave through its strip, 64 bytes of each at a time: lane l holds token l's values, and stores those of
+      // tokens l / 4 + 8 i, 16 bytes each.  (Straight from the registers, 16 bytes per token and instruction, with the addend's loads
+      // one behind the other: 10 us per tile.)
+      const int64_t t0 = (int64_t)tl.token * 256 + rank * 128 + quarter * 32;
+      uint8_t* strip = strips + warp * STRIP_BYTES;
+      uint4* own = reinterpret_cast<uint4*>(strip + lane * STRIP_PITCH);
+      uint4* dealt = reinterpret_cast<uint4*>(strip + (lane >> 2) * STRIP_PITCH + (lane & 3) * 16);  // token lane / 4 + 8 i: 8 i rows on
+      constexpr int kDealtStep = 8 * STRIP_PITCH / 16;
+      const int mine = (int)min((int64_t)32, p.T - t0) - (lane >> 2);  // of the four tokens, those with 8 i < mine are there
       if constexpr (GATED) {
         float amax = 0.f;
         auto activate = [&](auto activation) {
@@ -234,46 +247,78 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
           break;
         }
         amax = fmaxf(amax, am[128 * (piece ^ 1)]);
-        if (t < p.T) {
-          const float s = group_scale(amax), r = __frcp_rn(s);
-          uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + t * p.n + tl.w * 128 + piece * 64;
+        const float s = group_scale(amax), r = __frcp_rn(s);
 #pragma unroll
-          for (int c = 0; c < 64; c += 16) {
-            uint4 o;
-            uint32_t* word = reinterpret_cast<uint32_t*>(&o);
+        for (int c = 0; c < 64; c += 16) {
+          uint32_t word[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float v4[4] = {acc[c + 4 * q], acc[c + 4 * q + 1], acc[c + 4 * q + 2], acc[c + 4 * q + 3]};
-              word[q] = quant4(v4, s, r, amax <= 3.0e38f);
-            }
-            *reinterpret_cast<uint4*>(dst + c) = o;
+          for (int q = 0; q < 4; ++q) {
+            const float v4[4] = {acc[c + 4 * q], acc[c + 4 * q + 1], acc[c + 4 * q + 2], acc[c + 4 * q + 3]};
+            word[q] = quant4(v4, s, r, amax <= 3.0e38f);
           }
-          if (piece == 0) p.out_scale[t * (p.n / 128) + tl.w] = s;
+          own[c / 16] = make_uint4(word[0], word[1], word[2], word[3]);
         }
+        if (piece == 0 && t0 + lane < p.T) p.out_scale[(t0 + lane) * (p.n / 128) + tl.w] = s;
+        __syncwarp();
+        uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + (t0 + (lane >> 2)) * p.n + tl.w * 128 + piece * 64 + (lane & 3) * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (8 * i < mine) *reinterpret_cast<uint4*>(dst + 8 * i * p.n) = dealt[i * kDealtStep];
+        __syncwarp();
       } else {
         const int64_t ch0 = (int64_t)tl.w * 256 + piece * 128;
-        if (t < p.T) {
-          __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + t * p.n + ch0;
+        const int64_t at = (t0 + (lane >> 2)) * p.n + ch0 + (lane & 3) * 8;
+        const int cols = (int)min((int64_t)128, p.n - ch0);  // a multiple of 8, or nothing
+        uint4 more[4];
+        auto fetch = [&](int c) {  // the addend of 32 channels, as this lane will store them
 #pragma unroll
-          for (int c = 0; c < 128; c += 8) {
-            if (ch0 + c < p.n) {  // n is a multiple of 8
-              if (p.bias) {
-                const float4 b0 = __ldg(reinterpret_cast<const float4*>(p.bias + ch0 + c)), b1 = __ldg(reinterpret_cast<const float4*>(p.bias + ch0 + c + 4));
-                acc[c] += b0.x; acc[c + 1] += b0.y; acc[c + 2] += b0.z; acc[c + 3] += b0.w;
-                acc[c + 4] += b1.x; acc[c + 5] += b1.y; acc[c + 6] += b1.z; acc[c + 7] += b1.w;
-              }
-              if (p.addend) {
-                const uint4 raw = *reinterpret_cast<const uint4*>(p.addend + t * p.n + ch0 + c);
-                const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw);
+          for (int i = 0; i < 4; ++i)
+            if (8 * i < mine && c + (lane & 3) * 8 < cols) more[i] = *reinterpret_cast<const uint4*>(p.addend + at + 8 * i * p.n + c);
+        };
+        if (p.addend) fetch(0);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  acc[c + 2 * q] += __low2float(e[q]);
-                  acc[c + 2 * q + 1] += __high2float(e[q]);
+        for (int c = 0; c < 128; c += 32) {
+          if (c < cols) {
+            if (p.bias) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                if (c + j < cols) {
+                  const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + ch0 + c + j));
+                  acc[c + j] += b.x;
+                  acc[c + j + 1] += b.y;
+                  acc[c + j + 2] += b.z;
+                  acc[c + j + 3] += b.w;
                 }
               }
-              *reinterpret_cast<uint4*>(dst + c) = make_uint4(pack_bf16x2(acc[c], acc[c + 1]), pack_bf16x2(acc[c + 2], acc[c + 3]),
-                                                              pack_bf16x2(acc[c + 4], acc[c + 5]), pack_bf16x2(acc[c + 6], acc[c + 7]));
             }
+            if (p.addend) {  // to the lanes that hold the sums: they are added before the one rounding
+#pragma unroll
+              for (int i = 0; i < 4; ++i) dealt[i * kDealtStep] = more[i];
+              if (c + 32 < cols) fetch(c + 32);
+              __syncwarp();
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint4 raw = own[q];
+                const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  acc[c + 8 * q + 2 * u] += __low2float(e[u]);
+                  acc[c + 8 * q + 2 * u + 1] += __high2float(e[u]);
+                }
+              }
+              // a lane's own row: nobody else reads it before the next barrier
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float* v = acc + c + 8 * q;
+              own[q] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+            }
+            __syncwarp();
+            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + at + c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (8 * i < mine && c + (lane & 3) * 8 < cols) *reinterpret_cast<uint4*>(dst + 8 * i * p.n) = dealt[i * kDealtStep];
+            __syncwarp();
           }
         }
       }
@@ -301,12 +346,10 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
           }
           const uint32_t bar = bar_full0 + stage * 8, dst = ring + stage * STAGE_BYTES;
           if (weights) {
-            if constexpr (GATED) {
-              ptx::tma_load_2d_pair(dst + HALF_BYTES, &map_w, kb * KBYTES, tl.w * 128 + rank * 64, bar);
-              ptx::tma_load_2d_pair(dst + HALF_BYTES + HALF_BYTES / 2, &map_w, kb * KBYTES, (int)p.n + tl.w * 128 + rank * 64, bar);
-            } else {
-              ptx::tma_load_2d_pair(dst + HALF_BYTES, &map_w, kb * KBYTES, tl.w * 256 + rank * 128, bar);
-            }
+            // 64 rows for each half: 64 channels from here, or the same 64 channels' gate rows (CTA 0) and up rows
+            const int row = GATED ? tl.w * 128 + rank * (int)p.n : tl.w * 256 + rank * 64;
+            ptx::tma_load_2d_pair(dst + HALF_BYTES, &map_w, kb * KBYTES, row, bar);
+            ptx::tma_load_2d_pair(dst + HALF_BYTES + HALF_BYTES / 2, &map_w, kb * KBYTES, row + (GATED ? 64 : 128), bar);
           } else {
             if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
             ptx::tma_load_2d_pair(dst, &map_x, kb * KBYTES, tl.token * 256 + rank * 128, bar);
@@ -335,30 +378,34 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     if (rank == 0 && ptx::elect_one()) {
       const uint32_t ring = ptx::smem_u32(smem);
       const uint64_t da0 = ptx::smem_desc_sw128(ring), db0 = ptx::smem_desc_sw128(ring + HALF_BYTES);
-      constexpr uint32_t idesc = ptx::make_idesc(/*e4m3*/ 0, 256, 256);
+      constexpr uint32_t idesc = ptx::make_idesc(/*e4m3*/ 0, 256, 128);
       const uint16_t pair_mask = (uint16_t)(3 << cluster_rank);
       int stage = 0;
       uint32_t phase = 0, step = 0;
       bool alive = true;
       for (int i = worker; i < tiles && alive; i += workers) {
         for (int kb = kb0; kb < kb1; ++kb, ++step) {
-          const uint32_t buf = step & 1;
           if (!ptx::mbar_wait(&full_bar[stage], phase)) {
             report(0x2200 | stage);
             alive = false;
             break;
           }
-          if (!ptx::mbar_wait(&part_empty[buf], ((step >> 1) & 1) ^ 1)) {
-            report(0x2240 | buf);
-            alive = false;
-            break;
-          }
-          ptx::tc_fence_after_sync();
           const uint64_t off = (uint64_t)(stage * (STAGE_BYTES >> 4));
 #pragma unroll
-          for (int kk = 0; kk < KBYTES / 32; ++kk)
-            ptx::mma_f8f6f4_ss_pair(tmem_base + buf * 256, da0 + off + 2 * kk, db0 + off + 2 * kk, idesc, kk != 0);
-          ptx::mma_commit_both(&part_full[buf], pair_mask);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t buf = 2 * (step & 1) + h;
+            if (!ptx::mbar_wait(&part_empty[buf], ((step >> 1) & 1) ^ 1)) {
+              report(0x2240 | buf);
+              alive = false;
+              break;
+            }
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int kk = 0; kk < KBYTES / 32; ++kk)
+              ptx::mma_f8f6f4_ss_pair(tmem_base + buf * 128, da0 + off + 2 * kk, db0 + off + h * (HALF_BYTES / 2 >> 4) + 2 * kk, idesc, kk != 0);
+            ptx::mma_commit_both(&part_full[buf], pair_mask);
+          }
+          if (!alive) break;
           ptx::mma_commit_both(&empty_bar[stage], pair_mask);
           if (++stage == STAGES) {
             stage = 0;
@@ -478,7 +525,7 @@ int launch(const LinearParams& g, int split, cudaStream_t st) {
   if (rc) return rc;
   const cuuint64_t dims[2] = {(cuuint64_t)g.k, (cuuint64_t)w_rows};
   const cuuint64_t strides[1] = {(cuuint64_t)g.k};
-  const cuuint32_t box[2] = {KBYTES, GATED ? 64 : 128};
+  const cuuint32_t box[2] = {KBYTES, 64};
   rc = encode_tensor_map(&map_w, g.w, 1, 2, dims, strides, box, true, "weights");
   if (rc) return rc;
   KernelParams p;

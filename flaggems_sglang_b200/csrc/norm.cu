@@ -1,6 +1,7 @@
 // Residual addition, root-mean-square norm and quantisation to e4m3 in one pass over the rows:
 //     h = round(x + r);  y = h / sqrt(mean(h^2) + eps) * w;  q = e4m3(y / s), s = max(amax(y), 1e-10) / 448 per 128 channels
 //     (or one s per row), norm = round(y)
+// (quotients: rows.cuh)
 // A CTA owns a row at a time and keeps it in registers between the sum of squares and the outputs, so every byte is read and
 // written once: HBM bounds it from some ten MB on (beside the issue slots, where a row has neither residual nor norm to move), the
 // launch and the dependent reductions below that: one row of 7168 takes 3 us.
@@ -56,28 +57,6 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-
-// Division costs most instructions of this kernel where it is written as __fdiv_rn (42 per value in all, issue slots 74 % busy: 8192 rows of
-// 7168 in 93 us).  Here a quotient is a product with the reciprocal and one correction by its exact remainder, whose error is far below
-// half a unit in the last place; for the scale, whose divisor is a constant, that is the correctly rounded quotient for every significand
-// (all 2^23 compared), so that scales are the quantiser's bits.
-__device__ __forceinline__ float corrected(float v, float d, float r) {
-  const float q = v * r;
-  return fmaf(fmaf(-q, d, v), r, q);
-}
-__device__ __forceinline__ float scale_448(float amax) {
-  return amax <= 3.0e38f ? corrected(amax, 448.0f, 1.0f / 448.0f) : __fdiv_rn(amax, 448.0f);
-}
-// eight values over s -> e4m3
-__device__ __forceinline__ uint2 quant8_corrected(const float (&v)[8], float s, bool finite) {
-  if (!finite) return quant8(v, s, 0.f, false);
-  const float r = __fdividef(1.0f, s);
-  uint32_t half[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    half[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(corrected(v[2 * i], s, r), corrected(v[2 * i + 1], s, r)), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(half[0] | half[1] << 16, half[2] | half[3] << 16);
 }
 
 // Reduction over the CTA's warps, the same value in every thread.  `buf` holds a value per warp; two calls in a row use two.

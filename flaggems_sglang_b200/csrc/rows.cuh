@@ -50,7 +50,32 @@ __device__ __forceinline__ uint2 quant8(const float (&v)[8], float s, float r, b
   return make_uint2(lo, hi);
 }
 
-// Four values likewise.
+// Division costs most of the instructions of a quantiser that is written with __fdiv_rn (the norm: 42 per value in all, issue slots 74 %
+// busy, 93 us for 8192 rows of 7168).  Here a quotient is a product with the reciprocal and one correction by its exact remainder.  Its
+// error is 2^-23 of a unit in the last place before the rounding, so that it differs from the correctly rounded quotient at most where
+// that lies as close to the middle of two floats; by the constant 448 it is correctly rounded for every significand (all 2^23 compared),
+// so that scales are the same bits, and so are the e4m3 values of bf16 rows (all pairs of significands and 24 exponents compared).
+__device__ __forceinline__ float corrected_quotient(float v, float d, float r) {
+  const float q = v * r;
+  return fmaf(fmaf(-q, d, v), r, q);
+}
+// max / 448
+__device__ __forceinline__ float scale_448(float amax) {
+  return amax <= 3.0e38f ? corrected_quotient(amax, 448.0f, 1.0f / 448.0f) : __fdiv_rn(amax, 448.0f);
+}
+// eight values over s -> e4m3; `finite`: none of the group is infinite
+__device__ __forceinline__ uint2 quant8_corrected(const float (&v)[8], float s, bool finite) {
+  if (!finite) return quant8(v, s, 0.f, false);
+  const float r = __fdividef(1.0f, s);
+  uint32_t half[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    half[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(corrected_quotient(v[2 * i], s, r), corrected_quotient(v[2 * i + 1], s, r)),
+                                                 __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(half[0] | half[1] << 16, half[2] | half[3] << 16);
+}
+
+// Four values as quant8.
 __device__ __forceinline__ uint32_t quant4(const float (&v)[4], float s, float r, bool finite) {
   uint32_t w = 0;
   if (finite) {

@@ -177,6 +177,28 @@ def test_gated_mlp_of_bf16_rows_is_that_of_their_quantised_form():
     status()
 
 
+def test_quantised_bf16_rows_are_the_quantisers_for_every_significand():
+    """Every significand of a value over every one of the group's largest, 24 exponents apart at most, both signs: the quotients lie halfway
+    between two e4m3 values as often as bf16 allows.  Read back through a product with the identity."""
+    m = (128 + torch.arange(128, device="cuda")).float() / 128
+    rows_ = []
+    for d in range(0, 24, 1):
+        x = (m[None, :] * 2.0 ** -d).repeat(128, 1)  # row: the largest; column: the value
+        x = torch.where(torch.arange(128, device="cuda")[None] % 2 == 1, -x, x)
+        big = torch.cat([m[:, None] * 2, x[:, 1:]], 1)  # 2 m is larger than all values of the row
+        rows_ += [big, torch.cat([m[:, None] * 2, x[:, :1].expand(-1, 127)], 1)]
+    x = torch.cat(rows_).bfloat16()
+    assert (x.float().abs().amax(1) == x[:, 0].float()).all()
+    eye = torch.eye(128, device="cuda").to(torch.float8_e4m3fn)
+    one = torch.ones(1, 1, device="cuda")
+    xq, xs = quant(x)
+    for scale in (1.0, 2.0 ** -20, 2.0 ** 30):
+        a = fg().fp8_block_linear((x.float() * scale).bfloat16(), eye, one)
+        b = fg().fp8_block_linear(xq, eye, one, x_scale=xs * scale)
+        assert torch.equal(a, b)
+    status()
+
+
 def test_rows_do_not_depend_on_their_neighbours():
     """A row with NaN or infinity in it, or of zeros, leaves the other rows' bits alone; the rows behind the last are not there."""
     T, K, N = 37, 1024, 520
