@@ -133,6 +133,7 @@ SIGNATURES = {
     "fmoe_fp8_gate_up": (c_int, [POINTER(Fp8Args), c_void_p]),
     "fmoe_fp8_mlp_workspace_bytes": (c_int64, [POINTER(Fp8Args)]),
     "fmoe_fp8_mlp": (c_int, [POINTER(Fp8Args), c_void_p]),
+    "fmoe_debug_linear_kernel": (c_int, [c_int, c_int]),
     "fmoe_rms_norm_quant": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float,
                                     c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "fmoe_static_scratch_bytes": (c_int64, []),

@@ -5,23 +5,24 @@
 // The tensor cores cannot apply a scale inside their accumulator that changes with K, so every K block of 128 is multiplied into
 // a fresh TMEM partial (4 MMAs of K = 32) which the fold warps add, times a[t, kb] * b[n / 128, kb], to sums in registers.
 //
-//   tile    : 128 weight rows (gate/up: 128 gate rows and the same 128 up rows) on the MMA's M side x up to 16, 32, 64 or 128 tokens on
-//             N.  With the weights on M a call of one token costs a 16-column tile
-//   split   : S CTAs of a cluster share a tile, each with a contiguous part of its K blocks, so that few tiles still fill the
-//             chip.  Their sums meet through distributed shared memory, added in the order of the CTAs: the result does not
+//   tile    : 128 weight rows x up to 16, 32 or 64 tokens, the weights on the MMA's M side, so that one token costs a 16-column tile; or
+//             x up to 128 tokens with the tokens on M, where a fold thread owns a token and needs one factor per K block instead of one per
+//             column (128 tokens, 7168 x 4096, unsplit: 27 -> 18 us)
+//   gate/up : a tile is 128 channels, 64 gate rows and the same channels' up rows in each of two CTAs of the cluster
+//   split   : S CTAs (gate/up: S pairs) of a cluster share a tile, each with a contiguous part of its K blocks, so that few tiles still
+//             fill the chip.  Their sums meet through distributed shared memory, added in the order of the CTAs: the result does not
 //             depend on timing, and there is no scratch in global memory and no counter
-//   warps   : fold warps (TMEM lane quarter = warp % 4; 16 to 64 sums per thread), then TMA, MMA, and two that multiply token and weight
+//   warps   : fold warps (TMEM lane quarter = warp % 4; 16 or 32 sums per thread), then TMA, MMA, and two that multiply token and weight
 //             scales into a ring of factors
 //   batches : up to 32 tokens the partials of two or four K blocks are handed to the fold together.  What a K block costs there is not
-//             its FMAs but the chain wait - TMEM read - wait - hand back: 400 SM cycles each alone, 180 in batches of four (one token,
-//             7168 x 2048: 5.4 -> 4.9 us, gate/up of 7168 x 2 x 2048 10.5 -> 7.5 us)
+//             its FMAs but the chain wait - TMEM read - wait - hand back: 400 SM cycles each alone, 180 in batches of four
 //   epilogue: sums to shared memory [token][row], then a warp per token: a row of 128 channels is one coalesced store, and for
 //             gate/up it is one quantisation group, whose largest magnitude is a warp reduction
-// Two CTAs per SM for plain products of up to 32 tokens: twice as many clusters of 8 fit.  (Gate/up has eight fold warps; with two CTAs of
-// 384 threads an SM leaves 80 registers, and the fold takes twice as long as with one CTA and 141.)
+// Up to 32 tokens two CTAs share an SM: twice as many clusters of 8 fit.  (A register limit of 80 per thread, which two CTAs of 384 threads
+// or gate and up rows in one CTA bring, makes the fold take twice as long: 64 tokens 38 us for 56 K blocks against 17.7 with one CTA.)
 // Every mbarrier wait is bounded; the cluster barriers are reached by every thread on every path.
-// What bounds it: up to 64 tokens HBM beside the launch, the first loads and the join (one token, 7168 x 4096: 6.2 us, 4.7 TB/s); with 128
-// tokens what an SM takes in from L2, 32 KB per K block.
+// What bounds it: up to 64 tokens HBM beside the launch, the first loads and the join (one token, 7168 x 4096: 6.2 us, 4.7 TB/s; gate/up of
+// 7168 x 2 x 2048 6.9 us); with 128 tokens shared memory, 32 KB in and 32 KB of operands per K block (0.27 us).
 #include "linear.cuh"
 #include "pair.cuh"
 #include "rows.cuh"
@@ -44,27 +45,27 @@ constexpr int kSlots = 4;
 constexpr int kMaxSplit = 8;
 constexpr int BAR_BYTES = 512;
 
-// HALVES: 1 = plain, 2 = gate rows and up rows; COLS: most tokens of a tile; BATCH: K blocks whose partials are handed to the fold
-// together; ACC: sums per fold thread; CTAS: CTAs per SM
-template <int HALVES_, int COLS_, int BATCH_, int ACC_, int CTAS_>
+// COLS: most tokens of a tile; BATCH: K blocks whose partials are handed to the fold together; ACC: sums per fold thread; CTAS: CTAs per SM;
+// TOKENS_M: the tokens on M
+template <int COLS_, int BATCH_, int ACC_, int CTAS_, bool TOKENS_M_>
 struct Geo {
-  static constexpr int HALVES = HALVES_, COLS = COLS_, BATCH = BATCH_, ACC = ACC_, CTAS = CTAS_;
-  static constexpr int FOLD_WARPS = 4 * HALVES * (COLS / ACC);
+  static constexpr int COLS = COLS_, BATCH = BATCH_, ACC = ACC_, CTAS = CTAS_;
+  static constexpr bool TOKENS_M = TOKENS_M_;
+  static constexpr int FOLD_WARPS = 4 * (TOKENS_M ? 128 : COLS) / ACC;
   static constexpr int THREADS = (FOLD_WARPS + 4) * 32;
-  static constexpr int HALF_COLS = BATCH * COLS;        // TMEM columns of one half's partials
-  static constexpr int BUF_COLS = HALVES * HALF_COLS;
+  static constexpr int BUF_COLS = TOKENS_M ? 128 : BATCH * COLS;  // TMEM columns of a batch's partials
   static constexpr int BUFS = 512 / CTAS / BUF_COLS < 4 ? 512 / CTAS / BUF_COLS : 4;
   static constexpr int TMEM_COLS = BUFS * BUF_COLS;
-  static constexpr int STAGED = ACC > 32 ? 16 : BATCH * ACC;  // columns read from TMEM before the first is added
-  static constexpr int KB_FLOATS = HALVES * COLS;       // factors of one K block
-  static constexpr int SLOT_FLOATS = kGroup * KB_FLOATS;
-  static constexpr int FIXED_BYTES = BAR_BYTES + kSlots * SLOT_FLOATS * 4;
   // what a CTA takes, whatever its ring needs: so that neither a third CTA nor another TMEM kernel fits beside these, whose TMEM
   // allocation would wait for this one's end while a cluster of its own waits for it
   static constexpr int SMEM_BYTES = CTAS == 1 ? 227 * 1024 : 113 * 1024;
-  static constexpr int ROWS = 128 * HALVES;
-  static constexpr int SUM_BYTES = COLS * ROWS * 4;     // the sums, in place of the ring
-  static_assert(SUM_BYTES <= SMEM_BYTES - FIXED_BYTES && TMEM_COLS * CTAS <= 512 && kGroup % BATCH == 0, "shared memory, TMEM");
+  // the sums, in place of the ring; TOKENS_M: four floats of shift from token to token, for the 16-byte stores of its threads
+  static constexpr int SUM_PITCH = 128 + (TOKENS_M ? 4 : 0);
+  static constexpr int SUM_BYTES = COLS * SUM_PITCH * 4;
+  // factors of one K block: [gated: gate rows | up rows][token]
+  static constexpr int kb_floats(bool gated) { return (gated ? 2 : 1) * COLS; }
+  static constexpr int fixed_bytes(bool gated) { return BAR_BYTES + kSlots * kGroup * kb_floats(gated) * 4; }
+  static_assert(SUM_BYTES <= SMEM_BYTES - fixed_bytes(true) && TMEM_COLS * CTAS <= 512 && kGroup % BATCH == 0, "shared memory, TMEM");
 };
 
 struct KernelParams {
@@ -78,7 +79,7 @@ struct KernelParams {
   int kblocks;
   int token_tiles, token_tile;  // token_tile: a multiple of 16
   int stages, stage_bytes;
-  int split;      // CTAs per tile
+  int split;      // CTAs that share a tile's K blocks (gated: pairs of CTAs, each with half of the tile's channels)
   int activation;
   int early;      // the weights are complete when the kernel starts
 };
@@ -89,13 +90,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity));
 }
 
-template <typename G>
+template <typename G, bool GATED>
 __global__ void __launch_bounds__(G::THREADS, G::CTAS)
 fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const KernelParams p) {
-  constexpr int HALVES = G::HALVES, COLS = G::COLS, BATCH = G::BATCH;
+  constexpr int COLS = G::COLS, BATCH = G::BATCH, KB_FLOATS = G::kb_floats(GATED), SLOT_FLOATS = kGroup * KB_FLOATS;
   extern __shared__ __align__(1024) uint8_t smem[];
-  // barriers and factors first in the fixed part behind the ring; the ring itself starts at 0 (1024-byte aligned stages)
-  uint8_t* fixed = smem + G::SMEM_BYTES - G::FIXED_BYTES;
+  // barriers and factors behind the ring; the ring starts at 0 (1024-byte aligned stages: weights, then tokens)
+  uint8_t* fixed = smem + G::SMEM_BYTES - G::fixed_bytes(GATED);
   uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
   uint64_t* full_bar = bars;                    // [stages] TMA -> MMA
   uint64_t* empty_bar = bars + kMaxStages;      // [stages] MMA -> TMA
@@ -107,13 +108,14 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   float* factors = reinterpret_cast<float*>(fixed + BAR_BYTES);
 
   const int warp = ptx::uniform_warp_id(), lane = threadIdx.x & 31;
-  const int S = p.split;
-  const int rank = S > 1 ? (int)ptx::cluster_ctarank() : 0;
-  const int tile = (int)blockIdx.x / S;
+  const int S = p.split, ctas = GATED ? 2 * S : S;  // of a cluster
+  const int rank = ctas > 1 ? (int)ptx::cluster_ctarank() : 0;
+  const int slice = GATED ? rank >> 1 : rank, side = GATED ? rank & 1 : 0;  // part of K, half of the channels
+  const int tile = (int)blockIdx.x / ctas;
   const int row_tile = tile / p.token_tiles;
   const int tok0 = tile % p.token_tiles * p.token_tile;
-  const int kb0 = (int)((int64_t)p.kblocks * rank / S), kb1 = (int)((int64_t)p.kblocks * (rank + 1) / S);
-  const int up_tile = row_tile + (int)(p.n / 128);  // gate/up: the tile of up rows
+  const int kb0 = (int)((int64_t)p.kblocks * slice / S), kb1 = (int)((int64_t)p.kblocks * (slice + 1) / S);
+  const int up_tile = row_tile + (int)(p.n / 128);  // gated: the tile of up rows
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -147,15 +149,19 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     // ---------------- TMA producer ----------------
     if (ptx::elect_one()) {
       const uint32_t ring = ptx::smem_u32(smem);
-      const uint32_t bytes = HALVES * W_BYTES + p.token_tile * KBYTES;
+      const uint32_t bytes = W_BYTES + p.token_tile * KBYTES;
       auto load_weights = [&](int kb, int s) {
         const uint32_t dst = ring + s * p.stage_bytes, bar = ptx::smem_u32(&full_bar[s]);
         ptx::mbar_arrive_expect_tx(&full_bar[s], bytes);
-        ptx::tma_load_2d(dst, &map_w, kb * KBYTES, row_tile * 128, bar);
-        if constexpr (HALVES == 2) ptx::tma_load_2d(dst + W_BYTES, &map_w, kb * KBYTES, up_tile * 128, bar);
+        if constexpr (GATED) {  // 64 gate rows, then the same channels' up rows
+          ptx::tma_load_2d(dst, &map_w, kb * KBYTES, row_tile * 128 + side * 64, bar);
+          ptx::tma_load_2d(dst + W_BYTES / 2, &map_w, kb * KBYTES, up_tile * 128 + side * 64, bar);
+        } else {
+          ptx::tma_load_2d(dst, &map_w, kb * KBYTES, row_tile * 128, bar);
+        }
       };
       auto load_tokens = [&](int kb, int s) {
-        ptx::tma_load_2d(ring + s * p.stage_bytes + HALVES * W_BYTES, &map_x, kb * KBYTES, tok0, ptx::smem_u32(&full_bar[s]));
+        ptx::tma_load_2d(ring + s * p.stage_bytes + W_BYTES, &map_x, kb * KBYTES, tok0, ptx::smem_u32(&full_bar[s]));
       };
       int kb = kb0, stage = 0;
       uint32_t phase = 0;
@@ -199,8 +205,8 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       pdl_wait();
       pdl_trigger();
       const uint32_t ring = ptx::smem_u32(smem);
-      const uint64_t dw0 = ptx::smem_desc_sw128(ring), dx0 = ptx::smem_desc_sw128(ring + HALVES * W_BYTES);
-      const uint32_t idesc = ptx::make_idesc(/*e4m3*/ 0, 128, (uint32_t)p.token_tile);
+      const uint64_t dw0 = ptx::smem_desc_sw128(ring), dx0 = ptx::smem_desc_sw128(ring + W_BYTES);
+      const uint32_t idesc = ptx::make_idesc(/*e4m3*/ 0, 128, G::TOKENS_M ? 128 : (uint32_t)p.token_tile);
       int stage = 0;
       uint32_t phase = 0;
       const int steps = kb1 - kb0;
@@ -216,13 +222,10 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
         ptx::tc_fence_after_sync();
         const uint64_t off = (uint64_t)(stage * (p.stage_bytes >> 4));
-        const uint32_t to = tmem_base + buf * G::BUF_COLS + step % BATCH * COLS;
+        const uint32_t to = tmem_base + buf * G::BUF_COLS + (G::TOKENS_M ? 0 : step % BATCH * COLS);
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
-#pragma unroll
-          for (int kk = 0; kk < KBYTES / 32; ++kk)
-            ptx::mma_f8f6f4_ss(to + h * G::HALF_COLS, dw0 + off + h * (W_BYTES >> 4) + 2 * kk, dx0 + off + 2 * kk, idesc, kk != 0);
-        }
+        for (int kk = 0; kk < KBYTES / 32; ++kk)
+          ptx::mma_f8f6f4_ss(to, (G::TOKENS_M ? dx0 : dw0) + off + 2 * kk, (G::TOKENS_M ? dw0 : dx0) + off + 2 * kk, idesc, kk != 0);
         if (step % BATCH == BATCH - 1 || step == steps - 1) ptx::mma_commit(&part_full[buf]);
         ptx::mma_commit(&empty_bar[stage]);
         if (++stage == p.stages) {
@@ -239,9 +242,10 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     for (int g = me; g * kGroup < kb1 - kb0; g += 2) {
       const int first = kb0 + g * kGroup, count = min(kGroup, kb1 - first), slot = g % kSlots;
       constexpr int PER_LANE = (COLS + 31) / 32;
-      float a[PER_LANE][kGroup], b[HALVES][kGroup];
+      constexpr int ROW_BLOCKS = GATED ? 2 : 1;
+      float a[PER_LANE][kGroup], b[ROW_BLOCKS][kGroup];
 #pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
+      for (int h = 0; h < ROW_BLOCKS; ++h) {
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) b[h][i] = i < count ? __ldg(p.w_scale + (int64_t)(h ? up_tile : row_tile) * p.kblocks + first + i) : 0.f;
       }
@@ -256,26 +260,67 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         report(0x1300 | slot);
         break;
       }
-      float* dst = factors + slot * G::SLOT_FLOATS + lane;
+      float* dst = factors + slot * SLOT_FLOATS + lane;
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) {
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
+        for (int h = 0; h < ROW_BLOCKS; ++h) {
 #pragma unroll
           for (int j = 0; j < PER_LANE; ++j)
-            if (COLS % 32 == 0 || lane < COLS) dst[(i * HALVES + h) * COLS + 32 * j] = a[j][i] * b[h][i];
+            if (COLS % 32 == 0 || lane < COLS) dst[i * KB_FLOATS + h * COLS + 32 * j] = a[j][i] * b[h][i];
         }
       }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&sc_full[slot]);
     }
+  } else if constexpr (G::TOKENS_M) {
+    // ---------------- fold: a thread has a token, so one factor per half ----------------
+    pdl_entry_late();
+    constexpr int ACC = G::ACC;
+    static_assert(!G::TOKENS_M || ACC == 32, "one read per K block");
+    const int piece = warp >> 2, tok = (warp & 3) * 32 + lane;
+    const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + piece * ACC;
+    const float* mine = factors + (GATED ? piece >> 1 : 0) * COLS + tok;
+    float acc[ACC];
+#pragma unroll
+    for (int i = 0; i < ACC; ++i) acc[i] = 0.f;
+    const int steps = kb1 - kb0;
+    for (int step = 0; step < steps; ++step) {
+      const int buf = step % G::BUFS, g = step / kGroup, slot = g % kSlots;
+      if (step % kGroup == 0 && !warp_wait(&sc_full[slot], (g / kSlots) & 1)) {
+        report(0x1480 | slot);
+        break;
+      }
+      const float f = mine[slot * SLOT_FLOATS + step % kGroup * KB_FLOATS];
+      if (!warp_wait(&part_full[buf], (step / G::BUFS) & 1)) {
+        report(0x14c0 | buf);
+        break;
+      }
+      ptx::tc_fence_after_sync();
+      uint32_t v[32];
+      ptx::tmem_ld_32x32b_x32(from + buf * G::BUF_COLS, v);
+      ptx::tmem_ld_wait();
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      ptx::mbar_arrive_if(lane == 0, &part_empty[buf]);
+#pragma unroll
+      for (int i = 0; i < ACC; ++i) acc[i] = fmaf(__uint_as_float(v[i]), f, acc[i]);
+      if (step % kGroup == kGroup - 1 || step == steps - 1) ptx::mbar_arrive_if(lane == 0, &sc_empty[slot]);
+    }
+    // sums to shared memory, as below
+    float* sums = reinterpret_cast<float*>(smem) + tok * G::SUM_PITCH + piece * ACC;
+    if (tok < p.token_tile) {
+#pragma unroll
+      for (int i = 0; i < ACC; i += 4) *reinterpret_cast<float4*>(sums + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+    }
   } else {
     // ---------------- fold ----------------
     pdl_entry_late();
-    constexpr int ACC = G::ACC, STAGED = G::STAGED;
-    const int piece = warp >> 2, half = piece / (COLS / ACC), col0 = piece % (COLS / ACC) * ACC;
+    constexpr int ACC = G::ACC;
+    const int col0 = (warp >> 2) * ACC;
     const int cols = min(ACC, p.token_tile - col0);  // a multiple of 16, or nothing
-    const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + half * G::HALF_COLS + col0;
+    const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + col0;
+    const float* mine = factors + (GATED ? (warp & 3) >> 1 : 0) * COLS + col0;  // gated: lanes 0-63 hold gate rows
     float acc[ACC];
 #pragma unroll
     for (int i = 0; i < ACC; ++i) acc[i] = 0.f;
@@ -291,36 +336,28 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         break;
       }
       ptx::tc_fence_after_sync();
-      const float4* f4 = reinterpret_cast<const float4*>(factors + slot * G::SLOT_FLOATS + (step % kGroup * HALVES + half) * COLS + col0);
-      // The batch's columns, ACC of each K block in turn.  As many as registers allow are read before the first is waited for, and the
-      // partials are handed back before the FMAs: the MMAs of later K blocks run beside them.
+      const float* f = mine + slot * SLOT_FLOATS + step % kGroup * KB_FLOATS;
+      // The batch's columns, ACC of each K block in turn: all are read before the first is waited for, and the partials are handed back
+      // before the FMAs, so that the MMAs of later K blocks run beside them.
       constexpr int ALL = BATCH * ACC;
-      auto tok = [](int q) { return q % ACC; };
-      auto block = [](int q) { return q / ACC; };
-      auto there = [&](int q) { return block(q) < blocks && tok(q) < cols; };
+      auto there = [&](int q) { return q / ACC < blocks && q % ACC < cols; };
+      uint32_t v[ALL];
 #pragma unroll
-      for (int c = 0; c < ALL; c += STAGED) {
-        uint32_t v[STAGED];
+      for (int q = 0; q < ALL; q += 16)
+        if (there(q)) ptx::tmem_ld_32x32b_x16(from + buf * G::BUF_COLS + q / ACC * COLS + q % ACC, *reinterpret_cast<uint32_t(*)[16]>(v + q));
+      ptx::tmem_ld_wait();
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      ptx::mbar_arrive_if(lane == 0, &part_empty[buf]);
 #pragma unroll
-        for (int q = 0; q < STAGED; q += 16)
-          if (there(c + q))
-            ptx::tmem_ld_32x32b_x16(from + buf * G::BUF_COLS + block(c + q) * COLS + tok(c + q), *reinterpret_cast<uint32_t(*)[16]>(v + q));
-        ptx::tmem_ld_wait();
-        if (c + STAGED >= ALL) {
-          ptx::tc_fence_before_sync();
-          __syncwarp();
-          ptx::mbar_arrive_if(lane == 0, &part_empty[buf]);
-        }
-#pragma unroll
-        for (int q = 0; q < STAGED; q += 4) {
-          if (there(c + (q & ~15))) {
-            const float4 f = f4[block(c + q) * HALVES * (COLS / 4) + tok(c + q) / 4];
-            float* d = acc + tok(c + q);
-            d[0] = fmaf(__uint_as_float(v[q]), f.x, d[0]);
-            d[1] = fmaf(__uint_as_float(v[q + 1]), f.y, d[1]);
-            d[2] = fmaf(__uint_as_float(v[q + 2]), f.z, d[2]);
-            d[3] = fmaf(__uint_as_float(v[q + 3]), f.w, d[3]);
-          }
+      for (int q = 0; q < ALL; q += 4) {
+        if (there(q & ~15)) {
+          const float4 f4 = *reinterpret_cast<const float4*>(f + q / ACC * KB_FLOATS + q % ACC);
+          float* d = acc + q % ACC;
+          d[0] = fmaf(__uint_as_float(v[q]), f4.x, d[0]);
+          d[1] = fmaf(__uint_as_float(v[q + 1]), f4.y, d[1]);
+          d[2] = fmaf(__uint_as_float(v[q + 2]), f4.z, d[2]);
+          d[3] = fmaf(__uint_as_float(v[q + 3]), f4.w, d[3]);
         }
       }
       if (step % kGroup == kGroup - BATCH || step + BATCH >= steps) {
@@ -330,14 +367,14 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     }
     // Sums to shared memory in place of the ring: the last partial is complete, so every MMA has read its operands.  A warp
     // writes 32 consecutive rows of a token.
-    float* sums = reinterpret_cast<float*>(smem) + half * 128 + (warp & 3) * 32 + lane;
+    float* sums = reinterpret_cast<float*>(smem) + (warp & 3) * 32 + lane;
 #pragma unroll
     for (int i = 0; i < ACC; ++i)
-      if (i < cols) sums[(col0 + i) * G::ROWS] = acc[i];
+      if (i < cols) sums[(col0 + i) * G::SUM_PITCH] = acc[i];
   }
 
   ptx::tc_fence_before_sync();
-  if (S > 1) ptx::cluster_sync_all();
+  if (ctas > 1) ptx::cluster_sync_all();
   else __syncthreads();
   if (warp == G::FOLD_WARPS + 1) {
     ptx::tc_fence_after_sync();
@@ -346,18 +383,27 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
 
   // ---------------- epilogue: a warp per token, the tile's tokens dealt to the CTAs of the cluster ----------------
   const int tokens = (int)min((int64_t)p.token_tile, p.T - tok0);
-  join_tokens<HALVES, kMaxSplit>(rank + S * warp, S * (G::THREADS / 32), tokens, S, 0, 1, ptx::smem_u32(smem) + lane * 16, G::ROWS * 4,
-                                 [&](int t, float(&v)[HALVES][4]) {
-    const int64_t row = tok0 + t;
-    if constexpr (HALVES == 1) {
-      const int64_t ch = (int64_t)row_tile * 128 + lane * 4;
-      if (ch < p.n) store_plain(v[0], p.bias, p.addend, reinterpret_cast<__nv_bfloat16*>(p.out), row * p.n, ch);
-    } else {
+  const uint32_t sums = ptx::smem_u32(smem);
+  const int first = rank + ctas * warp, stride = ctas * (G::THREADS / 32);
+  if constexpr (GATED) {  // lanes 0-15 read the first half's channels, 16-31 the second's
+    join_tokens<2, kMaxSplit / 2>(first, stride, tokens, S, lane >> 4, 2, true, sums + (lane & 15) * 16, G::SUM_PITCH * 4, 256,
+                                  [&](int t, float(&v)[2][4]) {
+      const int64_t row = tok0 + t;
       store_gated(v, p.activation, reinterpret_cast<uint8_t*>(p.out) + row * p.n + row_tile * 128, p.out_scale + row * (p.n / 128) + row_tile);
-    }
-  });
-  if (S > 1) ptx::cluster_sync_all();  // nobody leaves while its sums are read
+    });
+  } else {
+    join_tokens<1, kMaxSplit>(first, stride, tokens, S, 0, 1, S > 1, sums + lane * 16, G::SUM_PITCH * 4, 0, [&](int t, float(&v)[1][4]) {
+      const int64_t ch = (int64_t)row_tile * 128 + lane * 4;
+      if (ch < p.n) store_plain(v[0], p.bias, p.addend, reinterpret_cast<__nv_bfloat16*>(p.out), (tok0 + t) * p.n, ch);
+    });
+  }
+  if (ctas > 1) ptx::cluster_sync_all();  // nobody leaves while its sums are read
 }
+
+using Few = Geo<16, 4, 16, 2, false>;
+using Some = Geo<32, 2, 32, 2, false>;
+using Half = Geo<64, 1, 32, 1, false>;
+using Many = Geo<128, 1, 32, 1, true>;
 
 // Clusters of 1 to 8 CTAs that the device holds at a time, by the CTAs per SM.  GPCs have different numbers of SMs, so that clusters of
 // 7 or 8 leave a fifth of them idle where a CTA takes a whole SM.
@@ -392,10 +438,8 @@ const Residents& residents() {
       return 0;
     };
     for (int s = 1; s <= kMaxSplit; ++s) {
-      using One = Geo<1, 64, 1, 32, 1>;
-      using Two = Geo<1, 16, 4, 16, 2>;
-      r.n[0][s] = ask((const void*)fp8_linear_kernel<One>, One::THREADS, One::SMEM_BYTES, s);
-      r.n[1][s] = ask((const void*)fp8_linear_kernel<Two>, Two::THREADS, Two::SMEM_BYTES, s);
+      r.n[0][s] = ask((const void*)fp8_linear_kernel<Many, false>, Many::THREADS, Many::SMEM_BYTES, s);
+      r.n[1][s] = ask((const void*)fp8_linear_kernel<Few, false>, Few::THREADS, Few::SMEM_BYTES, s);
       for (int c = 0; c < 2; ++c)
         if (r.n[c][s] == 0) r.n[c][s] = std::max(1, 148 * (c + 1) / s);
     }
@@ -406,24 +450,26 @@ const Residents& residents() {
 
 // The kernel and the number of CTAs (pair kernel: pairs) that share a tile's K blocks, by what the launch should take.  The models were
 // fitted to launches of K = 2048, 4096 and 7168, N = 512 to 7168 (gate/up: I = 768 to 3584) and 1 to 1024 tokens with every split; us:
-//   one CTA    rounds of clusters, each its K blocks at the slowest of the fold (0.18 to 0.95 by width), HBM's share of the weights and
+//   one CTA    rounds of clusters, each its K blocks at the slowest of the fold (0.18 to 0.28 by width), HBM's share of the weights and
 //              what an SM and the chip take in from L2, an epilogue, and the join of the sums
 //   CTA pairs  rounds of 0.38 per K block and the epilogue; shared tiles 0.44 and a longer one, as all sums cross shared memory
+// Of 126 such launches three took more than 1.1 times the best of all kernels and splits (4096 x 3584 gate/up of 24 tokens 8.1 us, 7.7 best).
 struct Choice {
   bool pair;
   int split;
 };
 
+thread_local Choice t_debug_choice{false, 0};  // fmoe_debug_linear_kernel
+
 Choice choose(const LinearParams& g, bool gated) {
   const Residents& r = residents();
-  const int halves = gated ? 2 : 1, kblocks = (int)(g.k / 128);
+  const int kblocks = (int)(g.k / 128);
   const int cols = g.T <= 16 ? 16 : (g.T <= 32 ? 32 : (g.T <= 64 ? 64 : 128));
-  const int ctas = !gated && cols <= 32 ? 2 : 1;
+  const int ctas = cols <= 32 ? 2 : 1, sides = gated ? 2 : 1;
   const int64_t token_tiles = ceil_div<int64_t>(g.T, cols), tiles = ceil_div<int64_t>(g.n, 128) * token_tiles;
   const double tokens = (double)(ceil_div<int64_t>(ceil_div<int64_t>(g.T, token_tiles), 16) * 16);
-  const double fold = cols == 128 ? (gated ? 0.31 + 0.005 * tokens : 0.28 + 0.0009 * tokens)
-                                  : (gated ? 0.24 + 0.003 * cols : 0.15 + 0.002 * cols);
-  const double bytes = halves * W_BYTES + tokens * KBYTES;
+  const double fold = cols == 128 ? 0.28 : 0.15 + 0.002 * cols;
+  const double bytes = W_BYTES + tokens * KBYTES;
   Choice best{false, 1};
   double best_us = 1e30;
   auto offer = [&](bool pair, int split, double us) {
@@ -432,47 +478,44 @@ Choice choose(const LinearParams& g, bool gated) {
       best = {pair, split};
     }
   };
-  for (int s = 1; s <= kMaxSplit && s <= kblocks; ++s) {
-    const int64_t at_once = r.n[ctas - 1][s], rounds = ceil_div<int64_t>(tiles, at_once);
-    const double active = (double)std::min<int64_t>(tiles, at_once) * s, per_sm = std::max(1.0, active / 148);
-    const double hbm = active * halves * W_BYTES / 8.0e6, l2 = std::max(bytes * per_sm / 1.0e5, active * bytes / 1.1e7);
+  for (int s = 1; s * sides <= kMaxSplit && s <= kblocks; ++s) {
+    const int64_t at_once = r.n[ctas - 1][s * sides], rounds = ceil_div<int64_t>(tiles, at_once);
+    const double active = (double)std::min<int64_t>(tiles, at_once) * s * sides, per_sm = std::max(1.0, active / 148);
+    const double hbm = active * W_BYTES / 8.0e6, l2 = std::max(bytes * per_sm / 1.2e5, active * bytes / 1.5e7);
     const double per_block = std::max(std::max(hbm, l2), fold * per_sm);
-    const double join = s == 1 ? 0.0 : (gated ? 0.4 + 0.1 * s + 0.022 * tokens : 0.2 + 0.05 * s + 0.013 * tokens);
-    offer(false, s, 2.0 + rounds * (0.7 + 0.01 * tokens * halves + ceil_div(kblocks, s) * per_block + join));
+    const double join = s == 1 ? 0.0 : 0.2 + 0.05 * s + (gated ? 0.004 : 0.013) * tokens;
+    offer(false, s, 2.0 + rounds * (0.7 + 0.01 * tokens + (gated ? 0.9 : 0.0) + (rounds > 1 ? 1.2 : 0.0) + ceil_div(kblocks, s) * per_block + join));
   }
   if (g.T > 64) {
     const int64_t pair_tiles = ceil_div<int64_t>(g.T, 256) * ceil_div<int64_t>(g.n, gated ? 128 : 256);
-    offer(true, 1, 3.0 + ceil_div<int64_t>(pair_tiles, r.n[0][2]) * (0.38 * kblocks + (gated ? 2.6 : 4.6)));
+    offer(true, 1, 3.0 + ceil_div<int64_t>(pair_tiles, r.n[0][2]) * (0.38 * kblocks + 3.0));
     for (int s = 2; s <= kMaxPairSplit && s <= kblocks; ++s)
       offer(true, s, 2.8 + ceil_div<int64_t>(pair_tiles, r.n[0][2 * s]) * (0.44 * ceil_div(kblocks, s) + 5.7));
   }
   return best;
 }
 
-template <typename G>
+template <typename G, bool GATED>
 int launch(const LinearParams& g, int split, cudaStream_t st) {
-  constexpr int HALVES = G::HALVES, COLS = G::COLS;
-  auto kernel = fp8_linear_kernel<G>;
+  auto kernel = fp8_linear_kernel<G, GATED>;
   static PerDeviceOnce once_attr;
   const cudaError_t attr_err = per_device_once(once_attr, [&] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES);
   });
   if (attr_err != cudaSuccess) return fail(FMOE_ERR_CUDA, "set-up of the e4m3 linear kernel failed: %s", cudaGetErrorString(attr_err));
   KernelParams p;
-  p.token_tiles = (int)ceil_div<int64_t>(g.T, COLS);
+  p.token_tiles = (int)ceil_div<int64_t>(g.T, G::COLS);
   p.token_tile = (int)(ceil_div<int64_t>(ceil_div<int64_t>(g.T, p.token_tiles), 16) * 16);
-  p.stage_bytes = HALVES * W_BYTES + p.token_tile * KBYTES;
-  p.stages = std::min(kMaxStages, (G::SMEM_BYTES - G::FIXED_BYTES) / p.stage_bytes);
+  p.stage_bytes = W_BYTES + (G::TOKENS_M ? G::COLS : p.token_tile) * KBYTES;  // TOKENS_M: lanes without tokens multiply what is there
+  p.stages = std::min(kMaxStages, (G::SMEM_BYTES - G::fixed_bytes(GATED)) / p.stage_bytes);
   p.kblocks = (int)(g.k / 128);
-  const int64_t row_tiles = ceil_div<int64_t>(g.n, 128);
   p.split = split;
-  const int64_t w_rows = HALVES * g.n;
   CUtensorMap map_x, map_w;
   int rc = pair_map_tokens(&map_x, g.x, g.T, g.k, 1, p.token_tile);
   if (rc) return rc;
-  const cuuint64_t dims[2] = {(cuuint64_t)g.k, (cuuint64_t)w_rows};
+  const cuuint64_t dims[2] = {(cuuint64_t)g.k, (cuuint64_t)(GATED ? 2 * g.n : g.n)};
   const cuuint64_t strides[1] = {(cuuint64_t)g.k};
-  const cuuint32_t box[2] = {KBYTES, 128};
+  const cuuint32_t box[2] = {KBYTES, GATED ? 64 : 128};
   rc = encode_tensor_map(&map_w, g.w, 1, 2, dims, strides, box, true, "weights");
   if (rc) return rc;
   p.x_scale = g.x_scale;
@@ -485,7 +528,9 @@ int launch(const LinearParams& g, int split, cudaStream_t st) {
   p.n = g.n;
   p.activation = g.activation;
   p.early = g.behind_late_trigger;
-  launch_pdl_cluster(kernel, p.split, dim3((unsigned)(row_tiles * p.token_tiles * p.split)), dim3(G::THREADS), G::SMEM_BYTES, st, map_x, map_w, p);
+  const int ctas = GATED ? 2 * split : split;
+  launch_pdl_cluster(kernel, ctas, dim3((unsigned)(ceil_div<int64_t>(g.n, 128) * p.token_tiles * ctas)), dim3(G::THREADS), G::SMEM_BYTES, st, map_x,
+                     map_w, p);
   return launch_status("fp8_linear_kernel");
 }
 
@@ -493,18 +538,20 @@ int launch(const LinearParams& g, int split, cudaStream_t st) {
 
 int run_linear(const LinearParams& p, bool gated, cudaStream_t st) {
   if (p.T <= 0) return FMOE_OK;
-  const Choice c = choose(p, gated);
-  if (c.pair) return run_linear_pair(p, gated, c.split, st);
-  if (gated) {
-    if (p.T <= 16) return launch<Geo<2, 16, 4, 16, 1>>(p, c.split, st);
-    if (p.T <= 32) return launch<Geo<2, 32, 2, 32, 1>>(p, c.split, st);
-    if (p.T <= 64) return launch<Geo<2, 64, 1, 32, 1>>(p, c.split, st);
-    return launch<Geo<2, 128, 1, 64, 1>>(p, c.split, st);
+  Choice c = choose(p, gated);
+  if (t_debug_choice.split > 0) {
+    c = t_debug_choice;
+    c.split = std::min(c.split, std::min((int)(p.k / 128), c.pair ? kMaxPairSplit : kMaxSplit / (gated ? 2 : 1)));
   }
-  if (p.T <= 16) return launch<Geo<1, 16, 4, 16, 2>>(p, c.split, st);
-  if (p.T <= 32) return launch<Geo<1, 32, 2, 32, 2>>(p, c.split, st);
-  if (p.T <= 64) return launch<Geo<1, 64, 1, 32, 1>>(p, c.split, st);
-  return launch<Geo<1, 128, 1, 32, 1>>(p, c.split, st);
+  if (c.pair) return run_linear_pair(p, gated, c.split, st);
+  auto go = [&](auto gated_c) {
+    constexpr bool GATED = decltype(gated_c)::value;
+    if (p.T <= 16) return launch<Few, GATED>(p, c.split, st);
+    if (p.T <= 32) return launch<Some, GATED>(p, c.split, st);
+    if (p.T <= 64) return launch<Half, GATED>(p, c.split, st);
+    return launch<Many, GATED>(p, c.split, st);
+  };
+  return gated ? go(std::true_type{}) : go(std::false_type{});
 }
 
 namespace {
@@ -625,6 +672,8 @@ int64_t workspace_bytes(const fmoe_fp8_args* a, Call call, const char* who) {
 
 }  // namespace
 
+void debug_linear_choice(bool pair, int split) { t_debug_choice = {pair, split}; }
+
 int status_word_linear_pair(int* out, bool clear);
 
 // of both kernels
@@ -658,4 +707,9 @@ extern "C" int64_t fmoe_fp8_mlp_workspace_bytes(const fmoe_fp8_args* args) {
 }
 extern "C" int fmoe_fp8_mlp(const fmoe_fp8_args* args, void* stream) {
   return fmoe::run_call(args, fmoe::Call::kMlp, "fp8_mlp", (cudaStream_t)stream);
+}
+extern "C" int fmoe_debug_linear_kernel(int pair, int split) {
+  FMOE_REQUIRE(split >= 0 && split <= fmoe::kMaxSplit, "debug_linear_kernel: split %d", split);
+  fmoe::debug_linear_choice(pair != 0, split);
+  return FMOE_OK;
 }

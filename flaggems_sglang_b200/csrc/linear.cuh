@@ -50,13 +50,14 @@ __device__ __forceinline__ void store_plain(float (&v)[4], const float* bias, co
   *reinterpret_cast<uint2*>(out + row_at + ch) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
-// The tokens first, first + stride, .. below `tokens` of a cluster's tile, by one warp: `parts` CTAs of the cluster (every `step`-th from
-// `from` on) hold sums of HALVES x 128 channels of each token, at the shared memory address base + pitch * token + 512 * half of their
-// own; they are added in the order of the CTAs and given to store(token, v), four channels of each half per lane.  Several tokens' sums
-// are on their way at a time: a read of another CTA's shared memory takes a few hundred cycles.
+// The tokens first, first + stride, .. below `tokens` of a cluster's tile, by one warp.  `parts` CTAs of the cluster (every step-th from
+// `from` on, which may differ from lane to lane; `remote`: there are others than this one) hold sums of a token, four channels of each of
+// HALVES for this lane, at the shared memory address base + pitch * token + apart * half of their own.  They are added in the order of the
+// CTAs and given to store(token, v).  Several tokens' sums are on their way at a time: a read of another CTA's shared memory takes a few
+// hundred cycles.
 template <int HALVES, int MOST, typename Store>
-__device__ __forceinline__ void join_tokens(int first, int stride, int tokens, int parts, int from, int step, uint32_t base, uint32_t pitch,
-                                            Store store) {
+__device__ __forceinline__ void join_tokens(int first, int stride, int tokens, int parts, int from, int step, bool remote, uint32_t base,
+                                            uint32_t pitch, uint32_t apart, Store store) {
   auto go = [&](auto parts_c) {
     constexpr int P = decltype(parts_c)::value, U = 8 / HALVES / P > 0 ? 8 / HALVES / P : 1;
     for (int t0 = first; t0 < tokens; t0 += stride * U) {
@@ -69,8 +70,8 @@ __device__ __forceinline__ void join_tokens(int first, int stride, int tokens, i
           if (s < parts) {
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
-              const uint32_t at = base + pitch * t + 512 * h;
-              part[u][s][h] = ptx::ld_cluster_f4(P > 1 ? ptx::mapa(at, from + step * s) : at);
+              const uint32_t at = base + pitch * t + apart * h;
+              part[u][s][h] = ptx::ld_cluster_f4(remote ? ptx::mapa(at, from + step * s) : at);
             }
           }
         }

@@ -203,8 +203,12 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       }
       if (!alive) break;
       if constexpr (SPLIT) {
-        // Sums to shared memory in place of the ring, [token][channel] (gate and up halves): the last partial is complete, so every
-        // MMA has read its operands.
+        // Sums to shared memory in place of the ring, [token][channel] (gate and up halves), once the last partials of both halves are
+        // complete: every MMA has read its operands then.
+        if (!warp_wait(&part_full[2 * ((step - 1) & 1) + (piece ^ 1)], ((step - 1) >> 1) & 1)) {
+          report(0x2480);
+          break;
+        }
         float* sums = reinterpret_cast<float*>(smem) + (quarter * 32 + lane) * SUM_PITCH;
 #pragma unroll
         for (int c = 0; c < 128; c += 4)
@@ -484,8 +488,8 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     const int tokens = (int)max((int64_t)0, min((int64_t)128, p.T - t0));
     // (the fold warps: the others have given their registers away)
     if (warp < kFoldWarps) {
-      join_tokens<2, kMaxSplit>((cluster_rank >> 1) + S * warp, S * kFoldWarps, tokens, S, rank, 2, ptx::smem_u32(smem) + lane * 16,
-                                SUM_PITCH * 4, [&](int t, float(&v)[2][4]) {
+      join_tokens<2, kMaxSplit>((cluster_rank >> 1) + S * warp, S * kFoldWarps, tokens, S, rank, 2, true, ptx::smem_u32(smem) + lane * 16,
+                                SUM_PITCH * 4, 512, [&](int t, float(&v)[2][4]) {
         if constexpr (GATED) {
           store_gated(v, p.activation, reinterpret_cast<uint8_t*>(p.out) + (t0 + t) * p.n + tl.w * 128,
                       p.out_scale + (t0 + t) * (p.n / 128) + tl.w);

@@ -80,6 +80,18 @@ def check(out, xv, wv, more=None):
     assert (off <= allowed).all(), f"off by {float((off - allowed).max())} more than allowed at {(off > allowed).nonzero()[:4].tolist()}"
 
 
+@pytest.fixture(params=["auto", "cta 1", "cta 3", "cta 8", "pair 1", "pair 2", "pair 3", "pair 4"])
+def kernel(request):
+    """Every kernel and split, whatever the library would choose for the shape."""
+    from flaggems_sglang_b200 import _C
+
+    if request.param != "auto":
+        which, split = request.param.split()
+        _C.check(_C.lib().fmoe_debug_linear_kernel(int(which == "pair"), int(split)))
+    yield request.param
+    _C.check(_C.lib().fmoe_debug_linear_kernel(0, 0))
+
+
 SHAPES = [
     # T, K, N: single token, one block, ragged widths; every token tile; K that does and does not divide among the CTAs of a tile
     (1, 128, 8), (1, 128, 128), (1, 7168, 2048), (2, 256, 136), (3, 384, 1000), (7, 1152, 576), (15, 2048, 4096), (16, 2048, 264),
@@ -90,22 +102,23 @@ SHAPES = [
 
 
 @pytest.mark.parametrize("T,K,N", SHAPES)
-def test_linear(T, K, N):
+def test_linear(T, K, N, kernel):
     xq, xs = quant(rows(T, K, T + K))
     w, ws = weight(N, K, N)
     out = fg().fp8_block_linear(xq, w, ws, x_scale=xs)
     assert out.shape == (T, N) and out.dtype == torch.bfloat16
     check(out, values(xq, xs), weight_values(w, ws))
-    again = fg().fp8_block_linear(xq, w, ws, x_scale=xs)
-    assert torch.equal(out.view(torch.int16), again.view(torch.int16)), "the result depends on timing"
+    for _ in range(3):
+        again = fg().fp8_block_linear(xq, w, ws, x_scale=xs)
+        assert torch.equal(out.view(torch.int16), again.view(torch.int16)), "the result depends on timing"
     status()
 
 
-@pytest.mark.parametrize("T,K,N", [(1, 256, 64), (5, 2048, 392), (70, 1024, 1000), (300, 896, 1544)])
+@pytest.mark.parametrize("T,K,N", [(1, 256, 64), (70, 1024, 1000), (300, 896, 1544)])
 @pytest.mark.parametrize("bias", [None, torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("addend", [False, True])
 @pytest.mark.parametrize("x_dtype", ["bf16", "e4m3"])
-def test_linear_extras_and_inputs(T, K, N, bias, addend, x_dtype):
+def test_linear_extras_and_inputs(T, K, N, bias, addend, x_dtype, kernel):
     x = rows(T, K, 5).bfloat16()
     xq, xs = quant(x)
     w, ws = weight(N, K, 6)
@@ -140,7 +153,7 @@ MLP_SHAPES = [(1, 128, 128, 8), (1, 7168, 2048, 7168), (4, 2048, 768, 2048), (16
 
 @pytest.mark.parametrize("T,K,I,N", MLP_SHAPES)
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
-def test_gated_mlp(T, K, I, N, activation):
+def test_gated_mlp(T, K, I, N, activation, kernel):
     xq, xs = quant(rows(T, K, 11, wide=False))
     w13, s13 = weight(2 * I, K, 12)
     w2, s2 = weight(N, I, 13)
@@ -199,7 +212,7 @@ def test_quantised_bf16_rows_are_the_quantisers_for_every_significand():
     status()
 
 
-def test_rows_do_not_depend_on_their_neighbours():
+def test_rows_do_not_depend_on_their_neighbours(kernel):
     """A row with NaN or infinity in it, or of zeros, leaves the other rows' bits alone; the rows behind the last are not there."""
     T, K, N = 37, 1024, 520
     xq, xs = quant(rows(T, K, 31))
@@ -216,7 +229,7 @@ def test_rows_do_not_depend_on_their_neighbours():
     status()
 
 
-def test_output_rows_behind_the_last_are_left_alone():
+def test_output_rows_behind_the_last_are_left_alone(kernel):
     """Through the C entry point, into a buffer with rows behind the last token's and a neighbour in front."""
     from flaggems_sglang_b200 import _C
 
