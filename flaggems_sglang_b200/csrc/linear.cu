@@ -239,6 +239,12 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     // ---------------- factors: two warps take alternate groups of eight K blocks ----------------
     pdl_entry_late();
     const int me = warp - (G::FOLD_WARPS + 2);
+    if (!GATED && p.addend && me == 1) {  // on its way to L2 while the tile is multiplied: the tokens that this CTA will store
+      const int64_t ch = (int64_t)row_tile * 128;
+      const int lines = (int)(min((int64_t)128, p.n - ch) * 2 + 127) / 128;
+      for (int t = rank + ctas * lane; t < p.token_tile && tok0 + t < p.T; t += ctas * 32)
+        for (int l = 0; l < lines; ++l) prefetch_l2(reinterpret_cast<const uint8_t*>(p.addend + (tok0 + t) * p.n + ch) + 128 * l);
+    }
     for (int g = me; g * kGroup < kb1 - kb0; g += 2) {
       const int first = kb0 + g * kGroup, count = min(kGroup, kb1 - first), slot = g % kSlots;
       constexpr int PER_LANE = (COLS + 31) / 32;

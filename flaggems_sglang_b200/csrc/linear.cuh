@@ -29,6 +29,8 @@ int run_linear_pair(const LinearParams& p, bool gated, int split, cudaStream_t s
 int run_linear(const LinearParams& p, bool gated, cudaStream_t st);
 
 #if defined(__CUDACC__)
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // A warp stores 128 channels of a token, four of each lane from `ch` on: bias and addend join, one rounding.
 __device__ __forceinline__ void store_plain(float (&v)[4], const float* bias, const __nv_bfloat16* addend, __nv_bfloat16* out, int64_t row_at,
                                             int64_t ch) {

@@ -430,6 +430,12 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       const int t0 = tl.token * 256 + rank * 128 + lane;
       const int b0 = GATED ? tl.w : 2 * tl.w, b1 = GATED ? tl.w + (int)(p.n / 128) : min(2 * tl.w + 1, p.w_blocks - 1);
       const float* w_mine = p.w_scale + (int64_t)(lane & 1 ? b1 : b0) * p.kblocks;  // lanes 0-15: K block lane / 2, block lane % 2
+      if (!GATED && p.addend) {  // on its way to L2 while the tile is multiplied: all workers read theirs at about the same time
+        const int64_t t = tl.token * 256 + rank * 128, ch = (int64_t)tl.w * 256;
+        const int lines = (int)(min((int64_t)256, p.n - ch) * 2 + 127) / 128;
+        for (int r = lane; r < 128 && t + r < p.T; r += 32)
+          for (int l = 0; l < lines; ++l) prefetch_l2(reinterpret_cast<const uint8_t*>(p.addend + (t + r) * p.n + ch) + 128 * l);
+      }
       for (int kb = kb0; kb < kb1; kb += kGroup, ++group) {
         const int slot = group % kSlots, count = min(kGroup, kb1 - kb);
         const float w = lane < 2 * count ? __ldg(w_mine + kb + (lane >> 1)) : 0.f;

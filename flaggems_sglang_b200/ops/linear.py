@@ -17,15 +17,25 @@ def _input(x: torch.Tensor, x_scale: torch.Tensor | None):
     T, K = x.shape
     if K == 0 or K % 128:
         raise ValueError(f"rows of {K} channels: a multiple of 128 is needed")
-    if x.dtype is torch.float8_e4m3fn:
-        if x_scale is None or x_scale.dtype is not torch.float32 or x_scale.shape != (T, K // 128):
-            raise ValueError("e4m3 x needs x_scale, fp32 [rows, K/128]")
-        return _aligned(x), x_scale if x_scale.is_contiguous() else x_scale.contiguous(), T, K, _C.E4M3
-    if x.dtype is not torch.bfloat16:
+    if not x.is_contiguous() or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    dtype = x.dtype
+    if dtype is torch.float8_e4m3fn:
+        _check_scale(x_scale, T, K, "e4m3 x needs x_scale, fp32 [rows, K/128]")
+        return x, x_scale if x_scale.is_contiguous() else x_scale.contiguous(), T, K, _C.E4M3
+    if dtype is not torch.bfloat16:
         raise ValueError("x must be bf16 or e4m3")
     if x_scale is not None:
         raise ValueError("x_scale belongs to e4m3 x")
-    return _aligned(x), None, T, K, _C.BF16
+    return x, None, T, K, _C.BF16
+
+
+def _check_scale(scale, rows: int, K: int, what: str) -> None:
+    if scale is not None and scale.dtype is torch.float32 and scale.dim() == 2:
+        r, k = scale.shape
+        if r == rows and k * 128 == K:
+            return
+    raise ValueError(what)
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -36,14 +46,15 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _weight(w: torch.Tensor, scale: torch.Tensor, K: int, name: str):
     """-> (weights, scales, N)"""
-    if w.dim() != 2 or w.dtype is not torch.float8_e4m3fn:
+    if w.dtype is not torch.float8_e4m3fn or w.dim() != 2:
         raise ValueError(f"{name} must be e4m3 [N, {K}]")
     N, k = w.shape
     if k != K or N == 0:
         raise ValueError(f"{name} must be e4m3 [N, {K}]")
-    if scale.dtype is not torch.float32 or scale.shape != ((N + 127) // 128, K // 128):
-        raise ValueError(f"the scales of {name} must be fp32 [ceil(N/128), {K // 128}]")
-    return _aligned(w), scale if scale.is_contiguous() else scale.contiguous(), N
+    _check_scale(scale, (N + 127) // 128, K, f"the scales of {name} must be fp32 [ceil(N/128), K/128]")
+    if not w.is_contiguous() or w.data_ptr() % 16:
+        w = w.clone(memory_format=torch.contiguous_format)
+    return w, scale if scale.is_contiguous() else scale.contiguous(), N
 
 
 def _bias(bias: torch.Tensor, N: int) -> torch.Tensor:
@@ -59,11 +70,12 @@ def _addend(addend: torch.Tensor, T: int, N: int) -> torch.Tensor:
 
 
 def _call(run, workspace_bytes, args: _C.Fp8Args, dev: torch.device) -> None:
+    """`workspace_bytes`: None where the call needs none."""
     if dev.index != _C.current_device():
         with _C.on_device(dev):
             return _call(run, workspace_bytes, args, dev)
-    need = workspace_bytes(args)
-    if need:
+    if workspace_bytes is not None:
+        need = workspace_bytes(args)
         if need < 0:
             _C.check(_C.ERR_INVALID_ARG)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -91,9 +103,9 @@ def fp8_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_
     out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
     if T:
         lib = _C.lib()
-        _call(lib.fmoe_fp8_linear, lib.fmoe_fp8_linear_workspace_bytes, _C.Fp8Args(
-            x_dtype=code, T=T, K=K, N=N, x=x.data_ptr(), x_scale=_C.ptr(x_scale), w=w.data_ptr(), w_scale=w_scale.data_ptr(),
-            bias=_C.ptr(bias), addend=_C.ptr(addend), out=out.data_ptr()), dev)
+        _call(lib.fmoe_fp8_linear, None if x_scale is not None else lib.fmoe_fp8_linear_workspace_bytes, _C.Fp8Args.of(
+            code, 0, 0, T, K, N, 0, x.data_ptr(), None if x_scale is None else x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), None, None,
+            None if bias is None else bias.data_ptr(), None if addend is None else addend.data_ptr(), out.data_ptr()), dev)
     return out
 
 
@@ -122,10 +134,9 @@ def fp8_gated_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w
     out = torch.empty(T, N, dtype=torch.bfloat16, device=dev)
     if T:
         lib = _C.lib()
-        _call(lib.fmoe_fp8_mlp, lib.fmoe_fp8_mlp_workspace_bytes, _C.Fp8Args(
-            x_dtype=code, activation=_C.ACTIVATIONS[activation], T=T, K=K, N=N, I=I, x=x.data_ptr(), x_scale=_C.ptr(x_scale),
-            w=w13.data_ptr(), w_scale=w13_scale.data_ptr(), w2=w2.data_ptr(), w2_scale=w2_scale.data_ptr(),
-            addend=_C.ptr(addend), out=out.data_ptr()), dev)
+        _call(lib.fmoe_fp8_mlp, lib.fmoe_fp8_mlp_workspace_bytes, _C.Fp8Args.of(
+            code, _C.ACTIVATIONS[activation], 0, T, K, N, I, x.data_ptr(), None if x_scale is None else x_scale.data_ptr(), w13.data_ptr(),
+            w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), None, None if addend is None else addend.data_ptr(), out.data_ptr()), dev)
     return out
 
 
