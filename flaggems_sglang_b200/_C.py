@@ -189,6 +189,26 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The module of csrc/host.cpp, bound to the loaded library; False where it has not been built for this torch (the operators then
+    take the longer way, through ctypes, to the same entry points)."""
+    global _host
+    if _host is None:
+        handle = lib()
+        try:
+            from . import _host as module
+        except ImportError:
+            _host = False
+        else:
+            module.bind(*(ctypes.cast(getattr(handle, "fmoe_" + name), c_void_p).value for name in (
+                "rms_norm_quant", "fp8_linear", "fp8_linear_workspace_bytes", "fp8_mlp", "fp8_mlp_workspace_bytes")))
+            _host = module
+    return _host
+
+
 def check(rc: int) -> None:
     if rc != OK:
         raise FmoeError(rc, lib().fmoe_last_error().decode("utf-8", "replace"))

@@ -4,6 +4,8 @@
 
 The library is a plain C-ABI shared object (see include/fmoe_b200.h); it links
 only the CUDA runtime.  Objects are rebuilt when a source or header is newer.
+Beside it _host.so is built from csrc/host.cpp, the short way from Python into some
+of the operators; it calls the library through the same C entry points.
 """
 from __future__ import annotations
 
@@ -47,6 +49,25 @@ def _deps_mtime() -> float:
     return max(os.path.getmtime(h) for h in hdrs)
 
 
+HOST_SRC = os.path.join(CSRC, "host.cpp")
+HOST_PATH = os.path.join(HERE, "_host.so")
+
+
+def _host_command() -> list[str]:
+    """The module with the short way into some of the operators: C++ against the torch and Python of this interpreter."""
+    import sysconfig
+
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    return [os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-I", sysconfig.get_paths()["include"], "-I", os.path.join(base, "include"),
+            "-I", os.path.join(base, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
+            HOST_SRC, "-o", HOST_PATH, "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+
+
 def ptxas_report(src: str) -> str:
     """Where the registers and spills of a source file's kernels are kept, as the compiler printed them."""
     return os.path.join(OBJ_DIR, src[:-3] + ".ptxas")
@@ -69,6 +90,14 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         return cmd, r
 
+    host_stale = force or not os.path.exists(HOST_PATH) or os.path.getmtime(HOST_PATH) < max(
+        os.path.getmtime(HOST_SRC), os.path.getmtime(os.path.join(INCLUDE, "fmoe_b200.h")))
+    if host_stale:
+        cmd, r = run(_host_command())
+        if verbose or r.returncode != 0:
+            sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+        if r.returncode != 0:
+            raise RuntimeError("compilation of csrc/host.cpp failed")
     if jobs:
         with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
             for cmd, r in ex.map(run, jobs):

@@ -5,11 +5,9 @@ import torch
 
 from .. import _C
 
-_ACTIVATIONS = ("silu", "gelu")
+_ACTIVATIONS = {name: _C.ACTIVATIONS[name] for name in ("silu", "gelu")}
 
 
-# A call on a few tokens lasts as long as these functions: attributes are read once, and tensors as they usually come (contiguous, 16-byte
-# aligned) are taken as they are.
 def _input(x: torch.Tensor, x_scale: torch.Tensor | None):
     """-> (rows, their scales or None, T, K, type code): bf16 rows that the call quantises, or e4m3 rows with a scale per 128 channels."""
     if x.dim() != 2:
@@ -91,6 +89,12 @@ def fp8_block_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_
     ``x_scale [T, K/128]`` as `rms_norm_quant_fp8` returns them.  Sums are fp32; ``bias [N]`` and ``addend [T, N]`` (bf16: a
     residual, another branch's output) join them before the one rounding.  K is a multiple of 128, N of 8.
     """
+    host = _C._host or _C.host()
+    if host:
+        out = host.linear(x, w, w_scale, x_scale, bias, addend)
+        if out is not None:
+            return out if type(out) is not int else _C.check(out)
+    # what is not dense, on another device, or refused
     dev = _C.require_cuda(x, w, w_scale, x_scale, bias, addend)
     x, x_scale, T, K, code = _input(x, x_scale)
     w, w_scale, N = _weight(w, w_scale, K, "w")
@@ -118,10 +122,16 @@ def fp8_gated_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w
     channels.  ``addend [T, N]`` (bf16) joins the sums: ``fp8_gated_mlp(..., addend=fused_moe(...))`` is the layer's output.
     K and I are multiples of 128, N of 8.
     """
+    code = _ACTIVATIONS.get(activation)
+    host = _C._host or _C.host()
+    if host and code is not None:
+        out = host.mlp(x, w13, w13_scale, w2, w2_scale, x_scale, code, addend)
+        if out is not None:
+            return out if type(out) is not int else _C.check(out)
     dev = _C.require_cuda(x, w13, w13_scale, w2, w2_scale, x_scale, addend)
-    if activation not in _ACTIVATIONS:
+    if code is None:
         raise ValueError(f"Unsupported activation: {activation}")
-    x, x_scale, T, K, code = _input(x, x_scale)
+    x, x_scale, T, K, x_code = _input(x, x_scale)
     w13, w13_scale, rows = _weight(w13, w13_scale, K, "w13")
     if rows % 256:
         raise ValueError(f"w13 has {rows} rows: 2I with I a multiple of 128 is needed")
@@ -135,7 +145,7 @@ def fp8_gated_mlp(x: torch.Tensor, w13: torch.Tensor, w13_scale: torch.Tensor, w
     if T:
         lib = _C.lib()
         _call(lib.fmoe_fp8_mlp, lib.fmoe_fp8_mlp_workspace_bytes, _C.Fp8Args.of(
-            code, _C.ACTIVATIONS[activation], 0, T, K, N, I, x.data_ptr(), None if x_scale is None else x_scale.data_ptr(), w13.data_ptr(),
+            x_code, code, 0, T, K, N, I, x.data_ptr(), None if x_scale is None else x_scale.data_ptr(), w13.data_ptr(),
             w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(), None, None if addend is None else addend.data_ptr(), out.data_ptr()), dev)
     return out
 

@@ -26,7 +26,12 @@ def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     y in x's type, for what reads the layer's input unquantised (a router, bf16 experts).
     K is a multiple of 128 (``per_token``: of 8), at most 16384.  Rows of x and residual may be strided; weight is bf16 or fp32 [K].
     """
-    # a call on a few rows lasts as long as this function: attributes are read once, the common layout is taken as it is
+    host = _C._host or _C.host()
+    if host:
+        got = host.norm(x, weight, eps, residual, per_token, return_norm)
+        if got is not None:
+            return got if type(got) is tuple else _C.check(got)
+    # what is not dense, on another device, or refused
     dev = _C.require_cuda(x, weight, residual)
     code, w_code = _CODES.get(x.dtype), _CODES.get(weight.dtype)
     if x.dim() != 2 or code is None:

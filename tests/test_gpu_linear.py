@@ -326,3 +326,55 @@ def test_refusals():
                 dict(w2=w2[:4], w2_scale=s2[:1])):
         with pytest.raises(ValueError):
             mlp(**{**dict(x=x, w13=w, w13_scale=ws, w2=w2, w2_scale=s2), **bad})
+
+
+def test_short_and_long_way_from_python_give_the_same(monkeypatch):
+    """Usual arguments go through the compiled module, others through ctypes: the same kernels, the same bits."""
+    from flaggems_sglang_b200 import _C
+
+    assert _C.host(), "the compiled module is not built"
+    T, K, I, N = 9, 512, 256, 328
+    x = rows(T, K, 91, wide=False).bfloat16()
+    xq, xs = quant(x)
+    w, ws = weight(N, K, 92)
+    w13, s13 = weight(2 * I, K, 93)
+    w2, s2 = weight(N, I, 94)
+    b, a = torch.randn(N, generator=gen(95), device="cuda"), torch.randn(T, N, generator=gen(96), device="cuda").bfloat16()
+
+    def results():
+        out = []
+        for extra in (dict(), dict(bias=b), dict(addend=a), dict(bias=b, addend=a)):
+            out += [fg().fp8_block_linear(x, w, ws, **extra), fg().fp8_block_linear(xq, w, ws, x_scale=xs, **extra)]
+        for extra in (dict(), dict(addend=a), dict(activation="gelu")):
+            out += [fg().fp8_gated_mlp(x, w13, s13, w2, s2, **extra), fg().fp8_gated_mlp(xq, w13, s13, w2, s2, x_scale=xs, **extra)]
+        for per_token in (False, True):
+            for keep in (False, True):
+                r = a[:, :K // 2].contiguous().repeat(1, 2)[:, :K].contiguous() if N >= K // 2 else None
+                out += [*(t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in fg().rms_norm_quant_fp8(
+                    x, torch.ones(K, device="cuda"), residual=r, per_token=per_token, return_norm=keep)), r]
+        return out
+
+    short = results()
+    monkeypatch.setattr(_C, "_host", False)
+    monkeypatch.setattr(_C, "host", lambda: False)
+    for s, l in zip(short, results()):
+        assert s.dtype == l.dtype and s.shape == l.shape and torch.equal(s, l)
+    status()
+
+
+def test_short_way_leaves_odd_arguments_to_the_long_one():
+    from flaggems_sglang_b200 import _C
+
+    host = _C.host()
+    w, ws = weight(256, 512, 97)
+    x = torch.zeros(4, 512, dtype=torch.bfloat16, device="cuda")
+    one = torch.ones(512, device="cuda")
+    assert host.linear(x, w, ws, None, None, None).shape == (4, 256)
+    for bad in ((x.cpu(), w, ws, None, None, None), (x[:, ::2], w, ws, None, None, None), (x, w[:, :256], ws, None, None, None),
+                (x, w, ws.double(), None, None, None), (x, w, ws, ws, None, None), (x[:0], w, ws, None, None, None), (3, w, ws, None, None, None),
+                (x, w, ws, None, torch.zeros(256, dtype=torch.bfloat16, device="cuda"), None), (x, w, ws, None, None, x), (x, w)):
+        assert host.linear(*bad) is None
+    assert host.norm(x, one, 1, None, False, False) is None and host.norm(x, one[:256], 1e-6, None, False, False) is None
+    assert host.norm(x.half(), one, 1e-6, None, False, False) is None and host.norm(x, one, 1e-6, x.float(), False, False) is None
+    assert len(host.norm(x, one, 1e-6, None, False, True)) == 3
+    assert host.mlp(x, w, ws, w, ws, None, 0, None) is None and host.mlp(x, w, ws, w, ws, None, "silu", None) is None
