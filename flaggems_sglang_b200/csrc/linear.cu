@@ -11,18 +11,20 @@
 //   gate/up : a tile is 128 channels, 64 gate rows and the same channels' up rows in each of two CTAs of the cluster
 //   split   : S CTAs (gate/up: S pairs) of a cluster share a tile, each with a contiguous part of its K blocks, so that few tiles still
 //             fill the chip.  Their sums meet through distributed shared memory, added in the order of the CTAs: the result does not
-//             depend on timing, and there is no scratch in global memory and no counter
+//             depend on timing, and there is no scratch in global memory and no counter.  Up to 64 tokens every CTA sends its sums to the
+//             ones that store them (st.async, one mbarrier there; against two cluster barriers and reading the others' memory one token
+//             of 7168 x 2048 4.7 -> 4.2 us, 16 tokens of 2048 x 7168 5.1 -> 4.2); 128 tokens have no room to land
 //   warps   : fold warps (TMEM lane quarter = warp % 4; 16 or 32 sums per thread), then TMA, MMA, and two that multiply token and weight
 //             scales into a ring of factors
 //   batches : up to 32 tokens the partials of two or four K blocks are handed to the fold together.  What a K block costs there is not
 //             its FMAs but the chain wait - TMEM read - wait - hand back: 400 SM cycles each alone, 180 in batches of four
-//   epilogue: sums to shared memory [token][row], then a warp per token: a row of 128 channels is one coalesced store, and for
+//   epilogue: a warp per token: a row of 128 channels is one coalesced store, and for
 //             gate/up it is one quantisation group, whose largest magnitude is a warp reduction
 // Up to 32 tokens two CTAs share an SM: twice as many clusters of 8 fit.  (A register limit of 80 per thread, which two CTAs of 384 threads
 // or gate and up rows in one CTA bring, makes the fold take twice as long: 64 tokens 38 us for 56 K blocks against 17.7 with one CTA.)
 // Every mbarrier wait is bounded; the cluster barriers are reached by every thread on every path.
 // What bounds it: up to 64 tokens HBM beside the launch, the first loads and the join (one token, 7168 x 4096: 6.2 us, 4.7 TB/s; gate/up of
-// 7168 x 2 x 2048 6.9 us); with 128 tokens shared memory, 32 KB in and 32 KB of operands per K block (0.27 us).
+// 7168 x 2 x 2048 7.1 us); with 128 tokens shared memory, 32 KB in and 32 KB of operands per K block (0.27 us).
 #include "linear.cuh"
 #include "pair.cuh"
 #include "rows.cuh"
@@ -59,12 +61,16 @@ struct Geo {
   // what a CTA takes, whatever its ring needs: so that neither a third CTA nor another TMEM kernel fits beside these, whose TMEM
   // allocation would wait for this one's end while a cluster of its own waits for it
   static constexpr int SMEM_BYTES = CTAS == 1 ? 227 * 1024 : 113 * 1024;
-  // the sums, in place of the ring; TOKENS_M: four floats of shift from token to token, for the 16-byte stores of its threads
+  // Sums: up to 64 tokens every CTA sends its own to the CTAs that store them, which have room for them beside the ring: 128 floats per
+  // token and sender.  TOKENS_M: they stay here, in place of the ring, four floats of shift from token to token for the 16-byte stores of
+  // the fold, and are read by the CTAs that store them.
+  static constexpr bool SENDS = !TOKENS_M;
   static constexpr int SUM_PITCH = 128 + (TOKENS_M ? 4 : 0);
-  static constexpr int SUM_BYTES = COLS * SUM_PITCH * 4;
+  static constexpr int LAND_BYTES = SENDS ? (COLS + kMaxSplit) * 512 : 0;
+  static constexpr int SUM_BYTES = SENDS ? 0 : COLS * SUM_PITCH * 4;
   // factors of one K block: [gated: gate rows | up rows][token]
   static constexpr int kb_floats(bool gated) { return (gated ? 2 : 1) * COLS; }
-  static constexpr int fixed_bytes(bool gated) { return BAR_BYTES + kSlots * kGroup * kb_floats(gated) * 4; }
+  static constexpr int fixed_bytes(bool gated) { return BAR_BYTES + LAND_BYTES + kSlots * kGroup * kb_floats(gated) * 4; }
   static_assert(SUM_BYTES <= SMEM_BYTES - fixed_bytes(true) && TMEM_COLS * CTAS <= 512 && kGroup % BATCH == 0, "shared memory, TMEM");
 };
 
@@ -104,8 +110,10 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   uint64_t* part_empty = part_full + 4;         // [BUFS] fold -> MMA
   uint64_t* sc_full = part_empty + 4;           // [kSlots] factor warps -> fold
   uint64_t* sc_empty = sc_full + kSlots;        // [kSlots] fold -> factor warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sc_empty + kSlots);
-  float* factors = reinterpret_cast<float*>(fixed + BAR_BYTES);
+  uint64_t* land_bar = sc_empty + kSlots;       // [1] sums of all CTAs -> epilogue
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(land_bar + 1);
+  uint8_t* land = fixed + BAR_BYTES;
+  float* factors = reinterpret_cast<float*>(land + G::LAND_BYTES);
 
   const int warp = ptx::uniform_warp_id(), lane = threadIdx.x & 31;
   const int S = p.split, ctas = GATED ? 2 * S : S;  // of a cluster
@@ -117,18 +125,24 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   const int kb0 = (int)((int64_t)p.kblocks * slice / S), kb1 = (int)((int64_t)p.kblocks * (slice + 1) / S);
   const int up_tile = row_tile + (int)(p.n / 128);  // gated: the tile of up rows
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      ptx::mbar_init(&full_bar[s], 1);
-      ptx::mbar_init(&empty_bar[s], 1);
+  const int tokens = (int)min((int64_t)p.token_tile, p.T - tok0);
+  const int mine = (tokens - rank + ctas - 1) / ctas;  // this CTA stores the tokens rank, rank + ctas, ..
+  if (threadIdx.x < 32) {
+    if (lane < p.stages) {
+      ptx::mbar_init(&full_bar[lane], 1);
+      ptx::mbar_init(&empty_bar[lane], 1);
     }
-    for (int b = 0; b < G::BUFS; ++b) {
-      ptx::mbar_init(&part_full[b], 1);
-      ptx::mbar_init(&part_empty[b], G::FOLD_WARPS);
+    if (lane < G::BUFS) {
+      ptx::mbar_init(&part_full[lane], 1);
+      ptx::mbar_init(&part_empty[lane], G::FOLD_WARPS);
     }
-    for (int s = 0; s < kSlots; ++s) {
-      ptx::mbar_init(&sc_full[s], 1);
-      ptx::mbar_init(&sc_empty[s], G::FOLD_WARPS);
+    if (lane < kSlots) {
+      ptx::mbar_init(&sc_full[lane], 1);
+      ptx::mbar_init(&sc_empty[lane], G::FOLD_WARPS);
+    }
+    if (lane == 0) {
+      ptx::mbar_init(land_bar, 1);
+      if (G::SENDS && ctas > 1) ptx::mbar_arrive_expect_tx(land_bar, mine * ctas * 512);
     }
     ptx::fence_barrier_init();
   }
@@ -143,6 +157,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   ptx::tc_fence_before_sync();
   __syncthreads();
   ptx::tc_fence_after_sync();
+  if (G::SENDS && ctas > 1) ptx::cluster_arrive();  // and waited for before the first sums are sent
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == G::FOLD_WARPS) {
@@ -371,16 +386,28 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         ptx::mbar_arrive_if(lane == 0, &sc_empty[slot]);
       }
     }
-    // Sums to shared memory in place of the ring: the last partial is complete, so every MMA has read its operands.  A warp
-    // writes 32 consecutive rows of a token.
-    float* sums = reinterpret_cast<float*>(smem) + (warp & 3) * 32 + lane;
+    // A warp has 32 consecutive rows of its tokens: through shared memory (in place of the ring: the last partial is complete, so every MMA
+    // has read its operands) into 16-byte pieces, and these to the CTA that stores the token, whose j-th token's sums from sender r are at
+    // land + (j * ctas + r) * 512.  (4 bytes at a time: 16 tokens 8.5 us where this takes 7.1.)
+    float* sums = reinterpret_cast<float*>(ctas > 1 ? smem : land) + (warp & 3) * 32;
 #pragma unroll
     for (int i = 0; i < ACC; ++i)
-      if (i < cols) sums[(col0 + i) * G::SUM_PITCH] = acc[i];
+      if (i < cols) sums[(col0 + i) * 128 + lane] = acc[i];
+    if (ctas > 1) {
+      __syncwarp();
+      ptx::cluster_wait();
+      const uint32_t to = ptx::smem_u32(land) + rank * 512 + ((warp & 3) * 32 + (lane & 7) * 4) * 4, bar = ptx::smem_u32(land_bar);
+      for (int t = col0 + (lane >> 3); t < min(col0 + cols, tokens); t += 4) {
+        const int j = t / ctas, owner = t - j * ctas;
+        ptx::st_async_f4(ptx::mapa(to + j * ctas * 512, owner), *reinterpret_cast<const float4*>(sums + t * 128 + (lane & 7) * 4),
+                         ptx::mapa(bar, owner));
+      }
+      __syncwarp();
+    }
   }
 
   ptx::tc_fence_before_sync();
-  if (ctas > 1) ptx::cluster_sync_all();
+  if (!G::SENDS && ctas > 1) ptx::cluster_sync_all();
   else __syncthreads();
   if (warp == G::FOLD_WARPS + 1) {
     ptx::tc_fence_after_sync();
@@ -388,22 +415,53 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   }
 
   // ---------------- epilogue: a warp per token, the tile's tokens dealt to the CTAs of the cluster ----------------
-  const int tokens = (int)min((int64_t)p.token_tile, p.T - tok0);
-  const uint32_t sums = ptx::smem_u32(smem);
-  const int first = rank + ctas * warp, stride = ctas * (G::THREADS / 32);
-  if constexpr (GATED) {  // lanes 0-15 read the first half's channels, 16-31 the second's
-    join_tokens<2, kMaxSplit / 2>(first, stride, tokens, S, lane >> 4, 2, true, sums + (lane & 15) * 16, G::SUM_PITCH * 4, 256,
-                                  [&](int t, float(&v)[2][4]) {
-      const int64_t row = tok0 + t;
+  auto store = [&](int t, auto& v) {
+    const int64_t row = tok0 + t;
+    if constexpr (GATED) {
       store_gated(v, p.activation, reinterpret_cast<uint8_t*>(p.out) + row * p.n + row_tile * 128, p.out_scale + row * (p.n / 128) + row_tile);
-    });
-  } else {
-    join_tokens<1, kMaxSplit>(first, stride, tokens, S, 0, 1, S > 1, sums + lane * 16, G::SUM_PITCH * 4, 0, [&](int t, float(&v)[1][4]) {
+    } else {
       const int64_t ch = (int64_t)row_tile * 128 + lane * 4;
-      if (ch < p.n) store_plain(v[0], p.bias, p.addend, reinterpret_cast<__nv_bfloat16*>(p.out), (tok0 + t) * p.n, ch);
-    });
+      if (ch < p.n) store_plain(v[0], p.bias, p.addend, reinterpret_cast<__nv_bfloat16*>(p.out), row * p.n, ch);
+    }
+  };
+  constexpr int ROW_BLOCKS = GATED ? 2 : 1;
+  if constexpr (G::SENDS) {
+    if (ctas > 1) {
+      if (mine > 0 && !warp_wait(land_bar, 0)) {
+        report(0x1500);
+        warp_wait(land_bar, 0);  // nobody writes here after this CTA has left
+      }
+      if (warp >= G::FOLD_WARPS) ptx::cluster_wait();  // the warps that sent nothing complete the barrier of the beginning
+    }
+    // gated: the sums of 64 channels' gate and up rows come from every second sender; lanes 0-15 take the first half's, 16-31 the second's
+    const float* at = reinterpret_cast<const float*>(land) + (GATED ? (lane >> 4) * 128 + (lane & 15) * 4 : lane * 4);
+    for (int j = warp; j < mine; j += G::THREADS / 32) {
+      float v[ROW_BLOCKS][4];
+#pragma unroll
+      for (int h = 0; h < ROW_BLOCKS; ++h) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[h][q] = 0.f;
+      }
+      for (int s = 0; s < S; ++s) {  // in the order of the senders
+#pragma unroll
+        for (int h = 0; h < ROW_BLOCKS; ++h) {
+          const float4 part = *reinterpret_cast<const float4*>(at + (j * ctas + s * ROW_BLOCKS) * 128 + 64 * h);
+          v[h][0] += part.x;
+          v[h][1] += part.y;
+          v[h][2] += part.z;
+          v[h][3] += part.w;
+        }
+      }
+      store(rank + j * ctas, v);
+    }
+  } else {
+    const uint32_t sums = ptx::smem_u32(smem);
+    const int first = rank + ctas * warp, stride = ctas * (G::THREADS / 32);
+    if constexpr (GATED)  // as above
+      join_tokens<2, kMaxSplit / 2>(first, stride, tokens, S, lane >> 4, 2, true, sums + (lane & 15) * 16, G::SUM_PITCH * 4, 256, store);
+    else join_tokens<1, kMaxSplit>(first, stride, tokens, S, 0, 1, S > 1, sums + lane * 16, G::SUM_PITCH * 4, 0, store);
+    if (ctas > 1) ptx::cluster_sync_relaxed();  // nobody leaves while its sums are read
   }
-  if (ctas > 1) ptx::cluster_sync_all();  // nobody leaves while its sums are read
 }
 
 using Few = Geo<16, 4, 16, 2, false>;

@@ -508,7 +508,7 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         }
       });
     }
-    ptx::cluster_sync_all();  // nobody leaves while its sums are read
+    ptx::cluster_sync_relaxed();  // nobody leaves while its sums are read
   }
 }
 

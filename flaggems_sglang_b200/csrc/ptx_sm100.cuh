@@ -205,6 +205,21 @@ __device__ __forceinline__ void st_async_16(uint32_t dst, const int4& v, uint32_
                "r"(v.y), "r"(v.z), "r"(v.w), "r"(bar)
                : "memory");
 }
+// 16 bytes to shared memory of the cluster, counted by an mbarrier of the same CTA that expects them
+__device__ __forceinline__ void st_async_f4(uint32_t dst, const float4& v, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(dst), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w), "r"(bar)
+               : "memory");
+}
+// The two halves of a cluster barrier
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// A cluster barrier that orders no memory: for leaving after the last read of another CTA's shared memory, whose values have been used.
+// (The release of the other one also waits for earlier global stores: 1000 cycles behind an epilogue.)
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 // Tiled TMA loads into THIS CTA's shared memory whose completion bytes are credited to an mbarrier that may live in the
 // pair's other CTA (cluster-wide address).  Plain loads: one destination CTA.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const CUtensorMap* map, int32_t x, int32_t y,
