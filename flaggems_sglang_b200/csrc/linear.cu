@@ -20,6 +20,9 @@
 //             its FMAs but the chain wait - TMEM read - wait - hand back: 400 SM cycles each alone, 180 in batches of four
 //   epilogue: a warp per token: a row of 128 channels is one coalesced store, and for
 //             gate/up it is one quantisation group, whose largest magnitude is a warp reduction
+//   bf16    : tokens are quantised by this kernel's idle warps while the weights are on their way, where the rows of a CTA are few: every
+//             CTA of a row of tiles quantises them again, some 25 instructions per channel, against 2.2 us for a launch that does it once
+//             (one token of 7168 x 2048 6.6 -> 5.5 us, 8 tokens of 2048 x 7168 6.4 -> 5.7; 16 of these 6.5 -> 7.3, so they are not)
 // Up to 32 tokens two CTAs share an SM: twice as many clusters of 8 fit.  (A register limit of 80 per thread, which two CTAs of 384 threads
 // or gate and up rows in one CTA bring, makes the fold take twice as long: 64 tokens 38 us for 56 K blocks against 17.7 with one CTA.)
 // Every mbarrier wait is bounded; the cluster barriers are reached by every thread on every path.
@@ -76,6 +79,7 @@ struct Geo {
 
 struct KernelParams {
   const float* x_scale;
+  const __nv_bfloat16* x_bf16;  // QUANT
   const float* w_scale;
   const float* bias;
   const __nv_bfloat16* addend;
@@ -85,6 +89,7 @@ struct KernelParams {
   int kblocks;
   int token_tiles, token_tile;  // token_tile: a multiple of 16
   int stages, stage_bytes;
+  int token_bytes;  // QUANT: a K block of the tile's tokens
   int split;      // CTAs that share a tile's K blocks (gated: pairs of CTAs, each with half of the tile's channels)
   int activation;
   int early;      // the weights are complete when the kernel starts
@@ -96,7 +101,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity));
 }
 
-template <typename G, bool GATED>
+// QUANT: the tokens are bf16 and quantised here, into an area behind the ring that holds all K blocks of this CTA
+template <typename G, bool GATED, bool QUANT>
 __global__ void __launch_bounds__(G::THREADS, G::CTAS)
 fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const KernelParams p) {
   constexpr int COLS = G::COLS, BATCH = G::BATCH, KB_FLOATS = G::kb_floats(GATED), SLOT_FLOATS = kGroup * KB_FLOATS;
@@ -111,7 +117,8 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   uint64_t* sc_full = part_empty + 4;           // [kSlots] factor warps -> fold
   uint64_t* sc_empty = sc_full + kSlots;        // [kSlots] fold -> factor warps
   uint64_t* land_bar = sc_empty + kSlots;       // [1] sums of all CTAs -> epilogue
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(land_bar + 1);
+  uint64_t* quant_bar = land_bar + 1;           // [1] quantisers -> MMA, fold
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(quant_bar + 1);
   uint8_t* land = fixed + BAR_BYTES;
   float* factors = reinterpret_cast<float*>(land + G::LAND_BYTES);
 
@@ -142,6 +149,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     }
     if (lane == 0) {
       ptx::mbar_init(land_bar, 1);
+      if (QUANT) ptx::mbar_init(quant_bar, G::FOLD_WARPS + 2);
       if (G::SENDS && ctas > 1) ptx::mbar_arrive_expect_tx(land_bar, mine * ctas * 512);
     }
     ptx::fence_barrier_init();
@@ -160,11 +168,62 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   if (G::SENDS && ctas > 1) ptx::cluster_arrive();  // and waited for before the first sums are sent
   const uint32_t tmem_base = *tmem_slot;
 
+  if (!GATED && p.addend && warp == G::FOLD_WARPS + 3) {  // on its way to L2 while the tile is multiplied: the tokens that this CTA will store
+    pdl_wait();
+    const int64_t ch = (int64_t)row_tile * 128;
+    const int lines = (int)(min((int64_t)128, p.n - ch) * 2 + 127) / 128;
+    for (int t = rank + ctas * lane; t < p.token_tile && tok0 + t < p.T; t += ctas * 32)
+      for (int l = 0; l < lines; ++l) prefetch_l2(reinterpret_cast<const uint8_t*>(p.addend + (tok0 + t) * p.n + ch) + 128 * l);
+  }
+  if constexpr (QUANT) {
+    static_assert(!G::TOKENS_M, "built for up to 64 tokens");
+    // ---------------- tokens: eight lanes own a group of 128 channels, all warps but those of TMA and MMA ----------------
+    if (warp < G::FOLD_WARPS || warp >= G::FOLD_WARPS + 2) {
+      pdl_entry_late();
+      constexpr int kIlp = 4, TEAMS = (G::FOLD_WARPS + 2) * 4;
+      const int sub = lane & 7, team = (warp < G::FOLD_WARPS ? warp : warp - 2) * 4 + (lane >> 3);
+      const int items = tokens * (kb1 - kb0);  // K block by K block
+      uint8_t* area = smem + p.stages * p.stage_bytes;
+      for (int first = team; __any_sync(0xffffffffu, first < items); first += TEAMS * kIlp) {
+        uint4 raw[kIlp][2];
+        float w[kIlp];  // of the weight block, in the lane that will write the factor
+        int at[kIlp], kbs[kIlp];
+#pragma unroll
+        for (int u = 0; u < kIlp; ++u) {
+          const int i = first + u * TEAMS;
+          kbs[u] = i / tokens;
+          at[u] = i - kbs[u] * tokens;
+          raw[u][0] = raw[u][1] = make_uint4(0, 0, 0, 0);
+          w[u] = 0.f;
+          if (i < items) {
+            const uint4* src = reinterpret_cast<const uint4*>(p.x_bf16 + ((tok0 + at[u]) * (int64_t)p.kblocks + kb0 + kbs[u]) * 128) + sub * 2;
+            raw[u][0] = __ldg(src);
+            raw[u][1] = __ldg(src + 1);
+            if (sub < (GATED ? 2 : 1)) w[u] = __ldg(p.w_scale + (int64_t)(sub ? up_tile : row_tile) * p.kblocks + kb0 + kbs[u]);
+          }
+        }
+        uint4 packed[kIlp];
+        float s[kIlp];
+        quant_groups(raw, packed, s);
+#pragma unroll
+        for (int u = 0; u < kIlp; ++u) {
+          if (first + u * TEAMS < items) {  // the swizzle of a 128-byte row: its 16-byte pieces exchanged by the row's number
+            *reinterpret_cast<uint4*>(area + kbs[u] * p.token_bytes + at[u] * KBYTES + ((sub ^ (at[u] & 7)) << 4)) = packed[u];
+            if (sub < (GATED ? 2 : 1)) factors[kbs[u] * KB_FLOATS + sub * COLS + at[u]] = s[u] * w[u];
+          }
+        }
+      }
+      ptx::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(quant_bar);
+    }
+  }
+
   if (warp == G::FOLD_WARPS) {
     // ---------------- TMA producer ----------------
     if (ptx::elect_one()) {
       const uint32_t ring = ptx::smem_u32(smem);
-      const uint32_t bytes = W_BYTES + p.token_tile * KBYTES;
+      const uint32_t bytes = QUANT ? W_BYTES : W_BYTES + p.token_tile * KBYTES;
       auto load_weights = [&](int kb, int s) {
         const uint32_t dst = ring + s * p.stage_bytes, bar = ptx::smem_u32(&full_bar[s]);
         ptx::mbar_arrive_expect_tx(&full_bar[s], bytes);
@@ -176,7 +235,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
       };
       auto load_tokens = [&](int kb, int s) {
-        ptx::tma_load_2d(ring + s * p.stage_bytes + W_BYTES, &map_x, kb * KBYTES, tok0, ptx::smem_u32(&full_bar[s]));
+        if constexpr (!QUANT) ptx::tma_load_2d(ring + s * p.stage_bytes + W_BYTES, &map_x, kb * KBYTES, tok0, ptx::smem_u32(&full_bar[s]));
       };
       int kb = kb0, stage = 0;
       uint32_t phase = 0;
@@ -220,11 +279,15 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       pdl_wait();
       pdl_trigger();
       const uint32_t ring = ptx::smem_u32(smem);
-      const uint64_t dw0 = ptx::smem_desc_sw128(ring), dx0 = ptx::smem_desc_sw128(ring + W_BYTES);
+      const uint64_t dw0 = ptx::smem_desc_sw128(ring), dx0 = ptx::smem_desc_sw128(ring + (QUANT ? p.stages * p.stage_bytes : W_BYTES));
       const uint32_t idesc = ptx::make_idesc(/*e4m3*/ 0, 128, G::TOKENS_M ? 128 : (uint32_t)p.token_tile);
       int stage = 0;
       uint32_t phase = 0;
-      const int steps = kb1 - kb0;
+      int steps = kb1 - kb0;
+      if (QUANT && !ptx::mbar_wait(quant_bar, 0)) {
+        report(0x1280);
+        steps = 0;
+      }
       for (int step = 0; step < steps; ++step) {
         const int batch = step / BATCH, buf = batch % G::BUFS;
         if (!ptx::mbar_wait(&full_bar[stage], phase)) {
@@ -236,11 +299,12 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
           break;
         }
         ptx::tc_fence_after_sync();
-        const uint64_t off = (uint64_t)(stage * (p.stage_bytes >> 4));
+        const uint64_t off = (uint64_t)(stage * (p.stage_bytes >> 4)), dw = dw0 + off;
+        const uint64_t dx = dx0 + (QUANT ? (uint64_t)(step * (p.token_bytes >> 4)) : off);
         const uint32_t to = tmem_base + buf * G::BUF_COLS + (G::TOKENS_M ? 0 : step % BATCH * COLS);
 #pragma unroll
         for (int kk = 0; kk < KBYTES / 32; ++kk)
-          ptx::mma_f8f6f4_ss(to, (G::TOKENS_M ? dx0 : dw0) + off + 2 * kk, (G::TOKENS_M ? dw0 : dx0) + off + 2 * kk, idesc, kk != 0);
+          ptx::mma_f8f6f4_ss(to, (G::TOKENS_M ? dx : dw) + 2 * kk, (G::TOKENS_M ? dw : dx) + 2 * kk, idesc, kk != 0);
         if (step % BATCH == BATCH - 1 || step == steps - 1) ptx::mma_commit(&part_full[buf]);
         ptx::mma_commit(&empty_bar[stage]);
         if (++stage == p.stages) {
@@ -254,13 +318,7 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     // ---------------- factors: two warps take alternate groups of eight K blocks ----------------
     pdl_entry_late();
     const int me = warp - (G::FOLD_WARPS + 2);
-    if (!GATED && p.addend && me == 1) {  // on its way to L2 while the tile is multiplied: the tokens that this CTA will store
-      const int64_t ch = (int64_t)row_tile * 128;
-      const int lines = (int)(min((int64_t)128, p.n - ch) * 2 + 127) / 128;
-      for (int t = rank + ctas * lane; t < p.token_tile && tok0 + t < p.T; t += ctas * 32)
-        for (int l = 0; l < lines; ++l) prefetch_l2(reinterpret_cast<const uint8_t*>(p.addend + (tok0 + t) * p.n + ch) + 128 * l);
-    }
-    for (int g = me; g * kGroup < kb1 - kb0; g += 2) {
+    for (int g = me; !QUANT && g * kGroup < kb1 - kb0; g += 2) {
       const int first = kb0 + g * kGroup, count = min(kGroup, kb1 - first), slot = g % kSlots;
       constexpr int PER_LANE = (COLS + 31) / 32;
       constexpr int ROW_BLOCKS = GATED ? 2 : 1;
@@ -345,10 +403,14 @@ fp8_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     float acc[ACC];
 #pragma unroll
     for (int i = 0; i < ACC; ++i) acc[i] = 0.f;
-    const int steps = kb1 - kb0;
+    int steps = kb1 - kb0;
+    if (QUANT && !warp_wait(quant_bar, 0)) {  // all factors are there
+      report(0x15c0);
+      steps = 0;
+    }
     for (int step = 0; step < steps; step += BATCH) {
       const int batch = step / BATCH, buf = batch % G::BUFS, g = step / kGroup, slot = g % kSlots, blocks = min(BATCH, steps - step);
-      if (step % kGroup == 0 && !warp_wait(&sc_full[slot], (g / kSlots) & 1)) {
+      if (!QUANT && step % kGroup == 0 && !warp_wait(&sc_full[slot], (g / kSlots) & 1)) {
         report(0x1400 | slot);
         break;
       }
@@ -469,6 +531,10 @@ using Some = Geo<32, 2, 32, 2, false>;
 using Half = Geo<64, 1, 32, 1, false>;
 using Many = Geo<128, 1, 32, 1, true>;
 
+// The query below counts one CTA per SM for every kernel that allocates TMEM, whatever it takes, so it is asked about this one, with the
+// others' shared memory and threads.
+__global__ void __launch_bounds__(Many::THREADS) stand_in_kernel() {}
+
 // Clusters of 1 to 8 CTAs that the device holds at a time, by the CTAs per SM.  GPCs have different numbers of SMs, so that clusters of
 // 7 or 8 leave a fifth of them idle where a CTA takes a whole SM.
 struct Residents {
@@ -484,8 +550,8 @@ const Residents& residents() {
   std::lock_guard<std::mutex> lock(mu);
   Residents& r = known[dev];
   if (!done[dev]) {
-    auto ask = [](const void* kernel, int threads, int smem, int split) {
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    auto ask = [](int threads, int smem, int split) {
+      cudaFuncSetAttribute(stand_in_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(split);
       cfg.blockDim = dim3(threads);
@@ -497,13 +563,13 @@ const Residents& residents() {
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0) return n;
+      if (cudaOccupancyMaxActiveClusters(&n, stand_in_kernel, &cfg) == cudaSuccess && n > 0) return n;
       cudaGetLastError();
       return 0;
     };
     for (int s = 1; s <= kMaxSplit; ++s) {
-      r.n[0][s] = ask((const void*)fp8_linear_kernel<Many, false>, Many::THREADS, Many::SMEM_BYTES, s);
-      r.n[1][s] = ask((const void*)fp8_linear_kernel<Few, false>, Few::THREADS, Few::SMEM_BYTES, s);
+      r.n[0][s] = ask(Many::THREADS, Many::SMEM_BYTES, s);
+      r.n[1][s] = ask(Few::THREADS, Few::SMEM_BYTES, s);
       for (int c = 0; c < 2; ++c)
         if (r.n[c][s] == 0) r.n[c][s] = std::max(1, 148 * (c + 1) / s);
     }
@@ -514,16 +580,39 @@ const Residents& residents() {
 
 // The kernel and the number of CTAs (pair kernel: pairs) that share a tile's K blocks, by what the launch should take.  The models were
 // fitted to launches of K = 2048, 4096 and 7168, N = 512 to 7168 (gate/up: I = 768 to 3584) and 1 to 1024 tokens with every split; us:
-//   one CTA    rounds of clusters, each its K blocks at the slowest of the fold (0.18 to 0.28 by width), HBM's share of the weights and
-//              what an SM and the chip take in from L2, an epilogue, and the join of the sums
+//   one CTA    rounds of clusters, each its K blocks at the slowest of the fold (0.19 to 0.28 by width), HBM's share of the weights and
+//              what an SM and the chip take in from L2, an epilogue, and the join of the sums; more than half the chip's room is dearer,
+//              as the next launch then cannot begin beside this one
+//   bf16 rows  2.2 for the quantiser's launch, or 0.9 (1.7 where CTAs share SMs) and 0.3 for every group of 128 channels that eight lanes
+//              quantise in the kernel; behind another launch of the same call clusters of 8 take 1.0 longer
 //   CTA pairs  rounds of 0.38 per K block and the epilogue; shared tiles 0.44 and a longer one, as all sums cross shared memory
-// Of 126 such launches three took more than 1.1 times the best of all kernels and splits (4096 x 3584 gate/up of 24 tokens 8.1 us, 7.7 best).
+// The choice is 1.01 times the best of all kernels and splits on average of 182 such launches, 1.1 times at worst; of 60 of bf16 rows too.
 struct Choice {
   bool pair;
   int split;
+  bool quant;  // the one-CTA kernel quantises bf16 tokens itself
 };
 
-thread_local Choice t_debug_choice{false, 0};  // fmoe_debug_linear_kernel
+thread_local Choice t_debug_choice{false, 0, false};  // fmoe_debug_linear_kernel
+
+int token_tile_of(int64_t T, int cols) {
+  const int64_t tiles = ceil_div<int64_t>(T, cols);
+  return (int)(ceil_div<int64_t>(ceil_div<int64_t>(T, tiles), 16) * 16);
+}
+
+// Stages of weights beside the quantised tokens of `slice` K blocks; 0: too few to keep the loads going, or no room for the factors
+template <typename G>
+int quant_stages(bool gated, int token_tile, int slice) {
+  const int token_bytes = token_tile * KBYTES;
+  if (slice > kSlots * kGroup) return 0;
+  const int stages = std::min(std::min(kMaxStages, slice), (G::SMEM_BYTES - G::fixed_bytes(gated) - slice * token_bytes) / W_BYTES);
+  return stages < std::min(slice, 4) ? 0 : stages;
+}
+bool can_quant(int64_t T, bool gated, int slice) {
+  if (T <= 16) return quant_stages<Few>(gated, 16, slice) > 0;
+  if (T <= 32) return quant_stages<Some>(gated, 32, slice) > 0;
+  return T <= 64 && quant_stages<Half>(gated, token_tile_of(T, 64), slice) > 0;
+}
 
 Choice choose(const LinearParams& g, bool gated) {
   const Residents& r = residents();
@@ -532,36 +621,41 @@ Choice choose(const LinearParams& g, bool gated) {
   const int ctas = cols <= 32 ? 2 : 1, sides = gated ? 2 : 1;
   const int64_t token_tiles = ceil_div<int64_t>(g.T, cols), tiles = ceil_div<int64_t>(g.n, 128) * token_tiles;
   const double tokens = (double)(ceil_div<int64_t>(ceil_div<int64_t>(g.T, token_tiles), 16) * 16);
-  const double fold = cols == 128 ? 0.28 : 0.15 + 0.002 * cols;
+  const double fold = cols == 128 ? 0.28 : 0.17 + 0.001 * cols;
   const double bytes = W_BYTES + tokens * KBYTES;
-  Choice best{false, 1};
+  Choice best{false, 1, false};
   double best_us = 1e30;
-  auto offer = [&](bool pair, int split, double us) {
+  auto offer = [&](bool pair, int split, double us, bool quant = false) {
     if (us < best_us) {
       best_us = us;
-      best = {pair, split};
+      best = {pair, split, quant};
     }
   };
+  const double before = g.x_bf16 ? 2.2 : 0.0;  // a quantiser's launch
   for (int s = 1; s * sides <= kMaxSplit && s <= kblocks; ++s) {
+    if (s == 7) continue;  // fits the GPCs badly: never more than 2 % better than another
     const int64_t at_once = r.n[ctas - 1][s * sides], rounds = ceil_div<int64_t>(tiles, at_once);
     const double active = (double)std::min<int64_t>(tiles, at_once) * s * sides, per_sm = std::max(1.0, active / 148);
-    const double hbm = active * W_BYTES / 8.0e6, l2 = std::max(bytes * per_sm / 1.2e5, active * bytes / 1.5e7);
+    const double hbm = active * W_BYTES / (gated ? 12.0e6 : 8.0e6), l2 = std::max(bytes * per_sm / 1.2e5, active * bytes / 1.5e7);
     const double per_block = std::max(std::max(hbm, l2), fold * per_sm);
-    const double join = s == 1 ? 0.0 : 0.2 + 0.05 * s + (gated ? 0.004 : 0.013) * tokens;
-    offer(false, s, 2.0 + rounds * (0.7 + 0.01 * tokens + (gated ? 0.9 : 0.0) + (rounds > 1 ? 1.2 : 0.0) + ceil_div(kblocks, s) * per_block + join));
+    const double join = s == 1 ? 0.0 : 0.2 + 0.05 * s + (gated ? 0.004 : 0.008) * tokens;
+    const double us = (active > 74 * ctas ? 2.4 : 2.0) + rounds * (0.7 + 0.01 * tokens + (gated ? 0.9 : 0.0) + (rounds > 1 ? 1.2 : 0.0) + ceil_div(kblocks, s) * per_block + join);
+    const bool wide = s == 8 && !gated;  // clusters that come in late while another launch leaves
+    offer(false, s, us + before + (wide && (g.x_bf16 || g.behind_late_trigger) ? 1.0 : 0.0));
+    if (g.x_bf16 && can_quant(g.T, gated, ceil_div(kblocks, s))) offer(false, s, us + rounds * ((active > 148 ? 1.7 : 0.9) + 0.3 * g.T * ceil_div(kblocks, s) / (cols == 64 ? 40 : 24)), true);
   }
   if (g.T > 64) {
     const int64_t pair_tiles = ceil_div<int64_t>(g.T, 256) * ceil_div<int64_t>(g.n, gated ? 128 : 256);
-    offer(true, 1, 3.0 + ceil_div<int64_t>(pair_tiles, r.n[0][2]) * (0.38 * kblocks + 3.0));
+    offer(true, 1, before + 3.0 + ceil_div<int64_t>(pair_tiles, r.n[0][2]) * (0.38 * kblocks + 3.0));
     for (int s = 2; s <= kMaxPairSplit && s <= kblocks; ++s)
-      offer(true, s, 2.8 + ceil_div<int64_t>(pair_tiles, r.n[0][2 * s]) * (0.44 * ceil_div(kblocks, s) + 5.7));
+      offer(true, s, before + 2.8 + ceil_div<int64_t>(pair_tiles, r.n[0][2 * s]) * (0.44 * ceil_div(kblocks, s) + 5.7));
   }
   return best;
 }
 
-template <typename G, bool GATED>
+template <typename G, bool GATED, bool QUANT>
 int launch(const LinearParams& g, int split, cudaStream_t st) {
-  auto kernel = fp8_linear_kernel<G, GATED>;
+  auto kernel = fp8_linear_kernel<G, GATED, QUANT>;
   static PerDeviceOnce once_attr;
   const cudaError_t attr_err = per_device_once(once_attr, [&] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES);
@@ -569,13 +663,21 @@ int launch(const LinearParams& g, int split, cudaStream_t st) {
   if (attr_err != cudaSuccess) return fail(FMOE_ERR_CUDA, "set-up of the e4m3 linear kernel failed: %s", cudaGetErrorString(attr_err));
   KernelParams p;
   p.token_tiles = (int)ceil_div<int64_t>(g.T, G::COLS);
-  p.token_tile = (int)(ceil_div<int64_t>(ceil_div<int64_t>(g.T, p.token_tiles), 16) * 16);
-  p.stage_bytes = W_BYTES + (G::TOKENS_M ? G::COLS : p.token_tile) * KBYTES;  // TOKENS_M: lanes without tokens multiply what is there
-  p.stages = std::min(kMaxStages, (G::SMEM_BYTES - G::fixed_bytes(GATED)) / p.stage_bytes);
+  p.token_tile = token_tile_of(g.T, G::COLS);
+  p.token_bytes = (G::TOKENS_M ? G::COLS : p.token_tile) * KBYTES;  // TOKENS_M: lanes without tokens multiply what is there
   p.kblocks = (int)(g.k / 128);
   p.split = split;
-  CUtensorMap map_x, map_w;
-  int rc = pair_map_tokens(&map_x, g.x, g.T, g.k, 1, p.token_tile);
+  p.x_bf16 = (const __nv_bfloat16*)g.x_bf16;
+  CUtensorMap map_x = {}, map_w;
+  int rc = 0;
+  if (QUANT) {
+    p.stage_bytes = W_BYTES;
+    p.stages = quant_stages<G>(GATED, p.token_tile, (int)ceil_div(p.kblocks, split));
+  } else {
+    p.stage_bytes = W_BYTES + p.token_bytes;
+    p.stages = std::min(kMaxStages, (G::SMEM_BYTES - G::fixed_bytes(GATED)) / p.stage_bytes);
+    rc = pair_map_tokens(&map_x, g.x, g.T, g.k, 1, p.token_tile);
+  }
   if (rc) return rc;
   const cuuint64_t dims[2] = {(cuuint64_t)g.k, (cuuint64_t)(GATED ? 2 * g.n : g.n)};
   const cuuint64_t strides[1] = {(cuuint64_t)g.k};
@@ -600,22 +702,34 @@ int launch(const LinearParams& g, int split, cudaStream_t st) {
 
 }  // namespace
 
-int run_linear(const LinearParams& p, bool gated, cudaStream_t st) {
+int run_linear(LinearParams p, bool gated, cudaStream_t st) {
   if (p.T <= 0) return FMOE_OK;
   Choice c = choose(p, gated);
   if (t_debug_choice.split > 0) {
     c = t_debug_choice;
-    c.split = std::min(c.split, std::min((int)(p.k / 128), c.pair ? kMaxPairSplit : kMaxSplit / (gated ? 2 : 1)));
+    const int kblocks = (int)(p.k / 128);
+    c.split = std::min(c.split, std::min(kblocks, c.pair ? kMaxPairSplit : kMaxSplit / (gated ? 2 : 1)));
+    c.quant = c.quant && p.x_bf16 && can_quant(p.T, gated, ceil_div(kblocks, c.split));
+  }
+  if (p.x_bf16 && !c.quant) {
+    const int rc = run_quant_tokens(p.x_bf16, p.T, p.k, p.xq, p.xq_scale, st);
+    if (rc) return rc;
+    p.x = p.xq;
+    p.x_scale = p.xq_scale;
+    p.behind_late_trigger = true;
   }
   if (c.pair) return run_linear_pair(p, gated, c.split, st);
-  auto go = [&](auto gated_c) {
-    constexpr bool GATED = decltype(gated_c)::value;
-    if (p.T <= 16) return launch<Few, GATED>(p, c.split, st);
-    if (p.T <= 32) return launch<Some, GATED>(p, c.split, st);
-    if (p.T <= 64) return launch<Half, GATED>(p, c.split, st);
-    return launch<Many, GATED>(p, c.split, st);
+  auto go = [&](auto gated_c, auto quant_c) {
+    constexpr bool GATED = decltype(gated_c)::value, QUANT = decltype(quant_c)::value;
+    if (p.T <= 16) return launch<Few, GATED, QUANT>(p, c.split, st);
+    if (p.T <= 32) return launch<Some, GATED, QUANT>(p, c.split, st);
+    if constexpr (QUANT) return launch<Half, GATED, QUANT>(p, c.split, st);
+    else return p.T <= 64 ? launch<Half, GATED, QUANT>(p, c.split, st) : launch<Many, GATED, QUANT>(p, c.split, st);
   };
-  return gated ? go(std::true_type{}) : go(std::false_type{});
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (c.quant) return gated ? go(Yes{}, Yes{}) : go(No{}, Yes{});
+  return gated ? go(Yes{}, No{}) : go(No{}, No{});
 }
 
 namespace {
@@ -713,11 +827,9 @@ int run_call(const fmoe_fp8_args* a, Call call, const char* who, cudaStream_t st
   if (!rc && call == Call::kMlp) rc = check_pointers(down, false, who);
   if (rc) return rc;
   if (a->x_dtype == FMOE_BF16) {
-    first.x = ws + at.xq;
-    first.x_scale = reinterpret_cast<float*>(ws + at.xs);
-    first.behind_late_trigger = true;
-    rc = run_quant_tokens(a->x, a->T, a->K, ws + at.xq, reinterpret_cast<float*>(ws + at.xs), st);
-    if (rc) return rc;
+    first.x_bf16 = a->x;
+    first.xq = ws + at.xq;
+    first.xq_scale = reinterpret_cast<float*>(ws + at.xs);
   } else {
     FMOE_REQUIRE(a->x_scale && (reinterpret_cast<uintptr_t>(a->x_scale) & 3u) == 0, "%s: e4m3 rows need x_scale", who);
     first.x = a->x;
@@ -736,7 +848,7 @@ int64_t workspace_bytes(const fmoe_fp8_args* a, Call call, const char* who) {
 
 }  // namespace
 
-void debug_linear_choice(bool pair, int split) { t_debug_choice = {pair, split}; }
+void debug_linear_choice(int kernel, int split) { t_debug_choice = {kernel == 1, split, kernel == 2}; }
 
 int status_word_linear_pair(int* out, bool clear);
 
@@ -772,8 +884,8 @@ extern "C" int64_t fmoe_fp8_mlp_workspace_bytes(const fmoe_fp8_args* args) {
 extern "C" int fmoe_fp8_mlp(const fmoe_fp8_args* args, void* stream) {
   return fmoe::run_call(args, fmoe::Call::kMlp, "fp8_mlp", (cudaStream_t)stream);
 }
-extern "C" int fmoe_debug_linear_kernel(int pair, int split) {
-  FMOE_REQUIRE(split >= 0 && split <= fmoe::kMaxSplit, "debug_linear_kernel: split %d", split);
-  fmoe::debug_linear_choice(pair != 0, split);
+extern "C" int fmoe_debug_linear_kernel(int kernel, int split) {
+  FMOE_REQUIRE(kernel >= 0 && kernel <= 2 && split >= 0 && split <= fmoe::kMaxSplit, "debug_linear_kernel: kernel %d, split %d", kernel, split);
+  fmoe::debug_linear_choice(kernel, split);
   return FMOE_OK;
 }

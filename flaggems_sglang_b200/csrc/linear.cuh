@@ -14,6 +14,9 @@ struct LinearParams {
   int64_t T = 0, n = 0, k = 0;
   const void* x = nullptr;         // [T, k] e4m3
   const float* x_scale = nullptr;  // [T, k/128]
+  const void* x_bf16 = nullptr;    // [T, k] instead of x and x_scale, quantised on the way: in the kernel, or to `xq` and `xq_scale` before it
+  void* xq = nullptr;
+  float* xq_scale = nullptr;
   const void* w = nullptr;
   const float* w_scale = nullptr;  // [ceil(rows/128), k/128]
   const float* bias = nullptr;     // [n]
@@ -26,7 +29,7 @@ struct LinearParams {
 };
 constexpr int kMaxPairSplit = 4;  // pairs that share a tile there
 int run_linear_pair(const LinearParams& p, bool gated, int split, cudaStream_t st);  // linear_pair.cu: many tokens
-int run_linear(const LinearParams& p, bool gated, cudaStream_t st);
+int run_linear(LinearParams p, bool gated, cudaStream_t st);
 
 #if defined(__CUDACC__)
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }

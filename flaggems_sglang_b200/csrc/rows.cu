@@ -209,28 +209,15 @@ quant_tokens_kernel(const uint4* __restrict__ x, int64_t items, uint4* __restric
         raw[u][1] = __ldg(x + i * 16 + sub * 2 + 1);
       }
     }
+    uint4 packed[kIlp];
+    float s[kIlp];
+    quant_groups(raw, packed, s);
 #pragma unroll
     for (int u = 0; u < kIlp; ++u) {
       const int64_t i = first + u * teams;
-      float v[2][8], amax = 0.f;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw[u][h]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[h][2 * j] = __low2float(e[j]);
-          v[h][2 * j + 1] = __high2float(e[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[h][j]));
-      }
-#pragma unroll
-      for (int off = 4; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
       if (i >= items) continue;
-      const float s = scale_448(fmaxf(amax, 1e-10f));
-      const uint2 lo = quant8_corrected(v[0], s, amax <= 3.0e38f), hi = quant8_corrected(v[1], s, amax <= 3.0e38f);
-      q[i * 8 + sub] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      if (sub == 0) scale[i] = s;
+      q[i * 8 + sub] = packed[u];
+      if (sub == 0) scale[i] = s[u];
     }
   }
 }

@@ -75,6 +75,57 @@ __device__ __forceinline__ uint2 quant8_corrected(const float (&v)[8], float s, 
   return make_uint2(half[0] | half[1] << 16, half[2] | half[3] << 16);
 }
 
+// U groups of 128 bf16 channels, 16 channels of each of eight neighbouring lanes: their e4m3 values, and the groups' scales in every lane.
+// All 32 lanes call it.  Step by step over all groups, and infinities are mended behind: a branch between them would put the groups'
+// dependent chains (shuffles, scale, reciprocal) one behind the other.
+template <int U>
+__device__ __forceinline__ void quant_groups(const uint4 (&raw)[U][2], uint4 (&packed)[U], float (&s)[U]) {
+  float amax[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw[u]);
+    __nv_bfloat162 m[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = __hmax2(__habs2(e[j]), __habs2(e[j + 4]));
+    m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+    amax[u] = fmaxf(__low2float(m[0]), __high2float(m[0]));
+  }
+#pragma unroll
+  for (int off = 4; off > 0; off >>= 1) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) amax[u] = fmaxf(amax[u], __shfl_xor_sync(0xffffffffu, amax[u], off));
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) s[u] = corrected_quotient(fmaxf(amax[u], 1e-10f), 448.0f, 1.0f / 448.0f);
+  auto value8 = [&](const uint4& part, float (&v)[8]) {
+    const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&part);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __low2float(e[j]);
+      v[2 * j + 1] = __high2float(e[j]);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float v[2][8];
+    value8(raw[u][0], v[0]);
+    value8(raw[u][1], v[1]);
+    const uint2 lo = quant8_corrected(v[0], s[u], true), hi = quant8_corrected(v[1], s[u], true);
+    packed[u] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (!(amax[u] <= 3.0e38f)) {
+      s[u] = scale_448(amax[u]);
+      float v[2][8];
+      value8(raw[u][0], v[0]);
+      value8(raw[u][1], v[1]);
+      const uint2 lo = quant8(v[0], s[u], 0.f, false), hi = quant8(v[1], s[u], 0.f, false);
+      packed[u] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+  }
+}
+
 // Four values as quant8.
 __device__ __forceinline__ uint32_t quant4(const float (&v)[4], float s, float r, bool finite) {
   uint32_t w = 0;

@@ -368,9 +368,10 @@ int64_t fmoe_fp8_gate_up_workspace_bytes(const fmoe_fp8_args* args);
 int fmoe_fp8_gate_up(const fmoe_fp8_args* args, void* stream);
 int64_t fmoe_fp8_mlp_workspace_bytes(const fmoe_fp8_args* args);
 int fmoe_fp8_mlp(const fmoe_fp8_args* args, void* stream);
-/* For tests: the calling thread's products take the one-CTA kernel (pair 0) or the CTA-pair kernel with each tile shared by up to `split`
- * of them, until a call with split 0 leaves the choice to the library again. */
-int fmoe_debug_linear_kernel(int pair, int split);
+/* For tests: the calling thread's products take the one-CTA kernel (0), the CTA-pair kernel (1) or the one-CTA kernel that quantises bf16
+ * rows itself, where it has room for them (2), with each tile shared by up to `split` CTAs or pairs, until a call with split 0 leaves the
+ * choice to the library again. */
+int fmoe_debug_linear_kernel(int kernel, int split);
 
 /*
  * Residual addition, root-mean-square norm and quantisation to e4m3 in one pass (no counterpart in the reference):

@@ -378,3 +378,37 @@ def test_short_way_leaves_odd_arguments_to_the_long_one():
     assert host.norm(x.half(), one, 1e-6, None, False, False) is None and host.norm(x, one, 1e-6, x.float(), False, False) is None
     assert len(host.norm(x, one, 1e-6, None, False, True)) == 3
     assert host.mlp(x, w, ws, w, ws, None, 0, None) is None and host.mlp(x, w, ws, w, ws, None, "silu", None) is None
+
+
+@pytest.mark.parametrize("split", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("T,K,N", [(1, 128, 64), (1, 7168, 264), (7, 1152, 1000), (16, 4096, 136), (17, 2048, 520), (32, 640, 1000),
+                                   (33, 1408, 264), (48, 2048, 1024), (64, 896, 120), (65, 512, 264), (97, 2048, 768), (128, 1024, 640),
+                                   (129, 640, 392), (300, 1152, 264)])
+def test_rows_quantised_in_the_product(T, K, N, split):
+    """bf16 rows that the product quantises itself give the bits that they give behind the quantiser's own launch."""
+    from flaggems_sglang_b200 import _C
+
+    x = rows(T, K, 31 * T + K).bfloat16()
+    x[T // 2, : GROUP // 2] = 0
+    x[T // 3, -GROUP:] = 0
+    w, ws = weight(N, K, N + 1)
+    I = -(-N // GROUP) * GROUP
+    w13, ws13 = weight(2 * I, K, N + 2)
+    w2, ws2 = weight(N, I, N + 3)
+    addend = torch.randn(T, N, generator=gen(5), device="cuda").bfloat16()
+    bias = torch.randn(N, generator=gen(6), device="cuda")
+    got = {}
+    try:
+        for which in (0, 2):
+            _C.check(_C.lib().fmoe_debug_linear_kernel(which, split))
+            got[which] = [fg().fp8_block_linear(x, w, ws, bias=bias, addend=addend), fg().fp8_gated_mlp(x, w13, ws13, w2, ws2, addend=addend)]
+            x2 = x.clone()
+            x2[0, 0], x2[-1, -1] = float("inf"), float("nan")
+            got[which].append(fg().fp8_block_linear(x2, w, ws))
+    finally:
+        _C.check(_C.lib().fmoe_debug_linear_kernel(0, 0))
+    for a, b in zip(got[0], got[2]):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    q, s = quant(x)
+    check(got[2][0], values(q, s), weight_values(w, ws), addend.float() + bias)
+    status()
