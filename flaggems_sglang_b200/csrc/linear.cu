@@ -799,6 +799,7 @@ int run_call(const fmoe_fp8_args* a, Call call, const char* who, cudaStream_t st
   int rc = lay_out(a, call, who, &first, &down);
   if (rc || a->T == 0) return rc;
   const Areas at(*a, call == Call::kMlp);
+  FMOE_REQUIRE(call != Call::kGateUp || (!a->bias && !a->addend), "%s: bias and addend join the last product of a call", who);
   FMOE_REQUIRE(a->x && aligned16(a->x), "%s: x is null or misaligned", who);
   FMOE_REQUIRE(at.total == 0 || (a->workspace && (reinterpret_cast<uintptr_t>(a->workspace) & 255u) == 0 && a->workspace_bytes >= at.total),
                "%s: the workspace is null, not 256-byte aligned or too small (%lld bytes given, %lld needed)", who,

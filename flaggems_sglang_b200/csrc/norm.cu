@@ -253,6 +253,17 @@ rms_norm_quant_stream_kernel(const NormParams p, int stages) {
   }
 }
 
+// Whether rows of K elements from a and from b have memory in common.  Interleaved rows of the same stride (halves of one buffer's) need
+// not, though the ranges from first to last do.
+bool rows_meet(const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t rows, int64_t K, int64_t size) {
+  const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));  // bytes
+  const int64_t a_len = ((rows - 1) * a_stride + K) * size, b_len = ((rows - 1) * b_stride + K) * size;
+  if (apart >= a_len || -apart >= b_len) return false;
+  if (rows == 1 || a_stride != b_stride) return true;
+  const int64_t pitch = a_stride * size, in_row = ((apart % pitch) + pitch) % pitch;
+  return in_row < K * size || in_row > pitch - K * size;
+}
+
 }  // namespace
 
 int status_word_norm(int* out, bool clear);
@@ -277,6 +288,9 @@ extern "C" int fmoe_rms_norm_quant(const void* x, int64_t x_stride, void* residu
   FMOE_REQUIRE(aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(norm) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0 &&
                    (reinterpret_cast<uintptr_t>(scale) & 3u) == 0,
                "rms_norm_quant: misaligned pointer");
+  FMOE_REQUIRE(!residual || (residual == x && residual_stride == x_stride) ||
+                   !rows_meet(x, x_stride, residual, residual_stride, rows, K, dtype == FMOE_BF16 ? 2 : 4),
+               "rms_norm_quant: residual shares memory with other rows of x");
   NormParams p{x, residual, weight, (uint8_t*)q, scale, norm, x_stride, residual_stride, rows, (int)K, weight_dtype == FMOE_F32, eps, 1.0f / (float)K};
   const int vecs = (int)(K / 8);
   const auto st = (cudaStream_t)stream;

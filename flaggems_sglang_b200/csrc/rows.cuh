@@ -88,7 +88,7 @@ __device__ __forceinline__ void quant_groups(const uint4 (&raw)[U][2], uint4 (&p
 #pragma unroll
     for (int j = 0; j < 4; ++j) m[j] = __hmax2(__habs2(e[j]), __habs2(e[j + 4]));
     m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
-    amax[u] = fmaxf(__low2float(m[0]), __high2float(m[0]));
+    amax[u] = fmaxf(fmaxf(__low2float(m[0]), __high2float(m[0])), 0.f);  // a group of nothing but NaN: as one of zeros
   }
 #pragma unroll
   for (int off = 4; off > 0; off >>= 1) {

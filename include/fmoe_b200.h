@@ -338,7 +338,7 @@ int fmoe_fused_experts_sorted(const fmoe_fused_args* args, const int32_t* topk_i
  *   K (and I) multiples of 128; partial sums are f32, the result is rounded once.
  * fmoe_fp8_linear : w has N rows (N a multiple of 8); out [T, N] bf16 = x w^T (+ bias [N] f32) (+ addend [T, N] bf16)
  * fmoe_fp8_gate_up: w has 2I rows (gate rows, then up rows; I a multiple of 128); h = act(x w_gate^T) * (x w_up^T) in f32, quantised
- *                   by the same rule: out [T, I] e4m3, out_scale [T, I/128] f32
+ *                   by the same rule: out [T, I] e4m3, out_scale [T, I/128] f32; no bias, no addend
  * fmoe_fp8_mlp    : both: h as above (it stays in the workspace), out [T, N] bf16 = h w2^T (+ bias) (+ addend); w2 [N, I] e4m3 with
  *                   w2_scale [ceil(N/128), I/128].  The shared expert of a layer, whose `addend` is the routed experts' result.
  * out may be addend itself, and otherwise overlaps no input.  The workspace (256-byte aligned) is used by one call at a time.
@@ -381,7 +381,8 @@ int fmoe_debug_linear_kernel(int kernel, int split);
  *   (scale [rows]); norm (optional) [rows, K]: y rounded to x's type
  * x, residual and norm are of `dtype` (FMOE_BF16 | FMOE_F32), weight [K] of weight_dtype (either).  x_stride and residual_stride are
  * elements from row to row (>= K; rows start at multiples of 16 bytes); q and norm are dense.  K a multiple of 128 (per_token: of 8),
- * at most 16384.  x may be residual itself; no other overlap of outputs and inputs.
+ * at most 16384.  x may be residual itself, or interleaved with it (halves of one buffer's rows); no
+ * other overlap of outputs and inputs.
  */
 int fmoe_rms_norm_quant(const void* x, int64_t x_stride, void* residual, int64_t residual_stride, int dtype, const void* weight,
                         int weight_dtype, int64_t rows, int64_t K, float eps, int per_token, void* q, float* scale, void* norm,

@@ -412,3 +412,52 @@ def test_rows_quantised_in_the_product(T, K, N, split):
     q, s = quant(x)
     check(got[2][0], values(q, s), weight_values(w, ws), addend.float() + bias)
     status()
+
+
+@pytest.mark.parametrize("T,K,N", [(262300, 128, 8200), (270000, 8192, 64)])
+def test_offsets_beyond_32_bits(T, K, N):
+    """More than 2^31 elements of output, or of input; the last rows, and the rows around element 2^31."""
+    x = torch.empty(T, K, dtype=torch.bfloat16, device="cuda")
+    for a in range(0, T, 30000):
+        x[a : a + 30000].normal_(generator=gen(a))
+    xq, xs = fg().per_token_group_quant_fp8(x)
+    del x
+    w, ws = weight(N, K, 3)
+    out = fg().fp8_block_linear(xq, w, ws, x_scale=xs)
+    middle = 2 ** 31 // max(K, N)
+    for part in (slice(T - 150, T), slice(middle - 70, middle + 70), slice(0, 50)):
+        check(out[part], values(xq[part], xs[part]), weight_values(w, ws))
+    status()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_offsets_beyond_32_bits_in_the_mlp(which):
+    """The last rows' bits are those of a call of their own, by the same kernel."""
+    from flaggems_sglang_b200 import _C
+
+    T, K, I, N = 530000, 256, 128, 4096  # 2.2 G elements of output
+    x = torch.empty(T, K, dtype=torch.bfloat16, device="cuda").normal_(generator=gen(1))
+    w13, s13 = weight(2 * I, K, 5)
+    w2, s2 = weight(N, I, 6)
+    try:
+        _C.check(_C.lib().fmoe_debug_linear_kernel(which, 1))
+        out = fg().fp8_gated_mlp(x, w13, s13, w2, s2)
+        part = slice(T - 130, T)
+        assert torch.equal(out[part], fg().fp8_gated_mlp(x[part], w13, s13, w2, s2))
+    finally:
+        _C.check(_C.lib().fmoe_debug_linear_kernel(0, 0))
+    status()
+
+
+def test_rows_of_nan_are_quantised_as_by_the_quantiser():
+    """A group of nothing but NaN has the smallest scale, and its values stay NaN; the other groups' products are lost with it, the other
+    rows' are not."""
+    x = rows(70, 256, 8, wide=False).bfloat16()
+    x[3, :GROUP] = float("nan")
+    w, ws = weight(264, 256, 9)
+    q, s = fg().per_token_group_quant_fp8(x)
+    want = fg().fp8_block_linear(q, w, ws, x_scale=s)
+    got = fg().fp8_block_linear(x, w, ws)
+    assert torch.isnan(got[3]).all()
+    keep = [t for t in range(70) if t != 3]
+    assert torch.equal(got[keep], want[keep])

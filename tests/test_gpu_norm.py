@@ -187,3 +187,35 @@ def test_norm_feeds_the_layer():
     rs.copy_(res0)
     graph.replay()
     assert torch.equal(again, out) and torch.equal(rs, h)
+
+
+def test_residual_beside_x():
+    """x and residual as halves of one buffer's rows, as one tensor, and as rows of one buffer one apart (refused)."""
+    both = torch.randn(9, 2 * 384, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").bfloat16()
+    w = torch.ones(384, device="cuda")
+    x, r = both[:, :384], both[:, 384:]
+    want_r = (x.float() + r.float()).bfloat16()
+    want = fg().rms_norm_quant_fp8(want_r, w)
+    keep = x.clone()
+    q, s = fg().rms_norm_quant_fp8(x, w, residual=r)
+    assert torch.equal(r, want_r) and torch.equal(x, keep)
+    assert torch.equal(q.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s, want[1])
+    same = keep.clone()
+    fg().rms_norm_quant_fp8(same, w, residual=same)
+    assert torch.equal(same, (keep.float() * 2).bfloat16())
+    rows = torch.zeros(9, 384, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="shares memory"):
+        fg().rms_norm_quant_fp8(rows[:-1], w, residual=rows[1:])
+
+
+def test_offsets_beyond_32_bits():
+    """2.2 G elements: the last rows are what they are in a call of their own."""
+    rows, K = 270000, 8192
+    x = torch.empty(rows, K, dtype=torch.bfloat16, device="cuda")
+    for a in range(0, rows, 30000):
+        x[a : a + 30000].normal_()
+    w = torch.ones(K, device="cuda")
+    tail = x[-300:].clone()
+    q, s = fg().rms_norm_quant_fp8(x, w)
+    q2, s2 = fg().rms_norm_quant_fp8(tail, w)
+    assert torch.equal(q[-300:].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s[-300:], s2)

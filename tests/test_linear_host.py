@@ -89,6 +89,24 @@ def test_norm_refuses(C):
     assert call(rows=0, x=None)[0] == C.OK
 
 
+def test_norm_refuses_a_residual_among_the_rows_of_x(C):
+    def call(r, rs=256, xs=256, rows=4, dtype=1, x=1 << 20):
+        rc = C.lib().fmoe_rms_norm_quant(x, xs, r, rs, dtype, 4096, 1, rows, 256, 1e-6, 0, 4096, 4096, None, None)
+        return rc, C.lib().fmoe_last_error().decode()
+
+    x = 1 << 20
+    # one row on, half a row on, before x, another stride, interleaved rows that overlap by 16 bytes, fp32
+    for kw in (dict(r=x + 512), dict(r=x + 256), dict(r=x - 512), dict(r=x - 16), dict(r=x, rs=512), dict(r=x + 496, rs=512, xs=512),
+               dict(r=x + 528, rs=512, xs=512), dict(r=x + 1024, dtype=0), dict(r=x + 16, rows=1)):
+        rc, msg = call(**kw)
+        assert rc == C.ERR_INVALID_ARG and "shares memory" in msg, (kw, msg)
+
+
+def test_gate_up_refuses_what_joins_a_last_product(C):
+    for name in ("bias", "addend"):
+        assert "join the last product" in bad_args(C, "fmoe_fp8_gate_up", x=4096, **{name: 4096})[1]
+
+
 def test_ops_refuse_cpu_tensors():
     import flaggems_sglang_b200 as fg
 
