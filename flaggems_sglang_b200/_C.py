@@ -201,6 +201,8 @@ def host():
         try:
             from . import _host as module
         except ImportError:
+            module = None
+        if module is None or module.torch_version != torch.__version__:
             _host = False
         else:
             module.bind(*(ctypes.cast(getattr(handle, "fmoe_" + name), c_void_p).value for name in (

@@ -62,7 +62,7 @@ def _host_command() -> list[str]:
     base = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
     return [os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DBUILT_FOR_TORCH="{torch.__version__}"',
             "-I", sysconfig.get_paths()["include"], "-I", os.path.join(base, "include"),
             "-I", os.path.join(base, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
             HOST_SRC, "-o", HOST_PATH, "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
@@ -90,9 +90,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         return cmd, r
 
+    import sysconfig
+
     host_stale = force or not os.path.exists(HOST_PATH) or os.path.getmtime(HOST_PATH) < max(
         os.path.getmtime(HOST_SRC), os.path.getmtime(os.path.join(INCLUDE, "fmoe_b200.h")))
-    if host_stale:
+    if host_stale and not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        sys.stderr.write("no Python.h: the operators of csrc/host.cpp are called through ctypes\n")
+    elif host_stale:
         cmd, r = run(_host_command())
         if verbose or r.returncode != 0:
             sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)

@@ -197,4 +197,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods};
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit__host() { return PyModule_Create(&module); }
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__host() {
+  if (Py_Version >> 16 != PY_VERSION_HEX >> 16) return PyErr_Format(PyExc_ImportError, "built for another version of Python");
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", BUILT_FOR_TORCH) < 0) Py_CLEAR(m);
+  return m;
+}
