@@ -8,14 +8,19 @@
 //               columns on their way: each 32 are replaced by the next as soon as they have been added, and the partial is handed back
 //               before the last 64 are.  The two halves' warps run half a K block apart, so that one's reads and waits are beside the
 //               other's FMAs
-//   warps 8, 9: TMA (tokens, weights)     warp 10: MMA (CTA 0)     warp 11: scales, eight K blocks at a time, transposed into a ring
+//   warp 8     : TMA of tokens and weights     warp 10: MMA (CTA 0)     warp 11: scales, eight K blocks at a time, transposed into a ring
+//   warp 9     : the addend into 64 KB of shared memory while the tile is multiplied, and the output from there, both by TMA.  The fold adds
+//                and rounds in place, so that a tile's stores run beside the next one's MMAs: with each warp's loads and stores from its
+//                registers 4096 x 2048 x 7168 with an addend took 91 us, this way 64; 8192 x 7168 x 4096 209 -> 193.  The ring gives up
+//                two of six stages for it, which costs nothing.
 // SPLIT: up to four pairs of a cluster share a tile's K blocks; their sums meet through distributed shared memory as in linear.cu.
 // What bounds it: up to some 1500 tokens about 800 clocks per K block and tile, of which shared memory (32 KB in, 48 KB of operands at 128
-// bytes per clock) needs 640 and what an SM takes in from L2 655; from there on the power limit (8192 x 7168 x 4096: 210 us, 2.3 PFLOP/s
+// bytes per clock) needs 640 and what an SM takes in from L2 655; from there on the power limit (8192 x 7168 x 4096: 193 us, 2.5 PFLOP/s
 // at about 1.5 GHz).  Tried: one MMA over all 256 rows of N (512 clocks of shared memory, but only two partials for the fold's round
 // trip: the same at 8192 tokens, 2048 x 2048 x 7168 42 us against 38); reads of the next K block before the last of this one are added
-// (30.5 us against 28.4 for one round of K = 7168).  An arrival behind a branch left the fold's warps split, so that each FMA was issued
-// twice: 247 us at 8192 tokens where it now takes 217 with the same epilogue.
+// (30.5 us against 28.4 for one round of K = 7168); 16 fold warps of 64 sums (223 us against 210 at 8192 tokens), packed FMAs (242), waits
+// that poll without a hint (251).  An arrival behind a branch left the fold's warps split, so that each FMA was issued twice: 247 us where
+// it then took 217.
 #include "linear.cuh"
 #include "pair.cuh"
 #include "rows.cuh"
@@ -34,7 +39,7 @@ namespace {
 constexpr int KBYTES = 128;
 constexpr int HALF_BYTES = 128 * KBYTES;          // this CTA's tokens, or weight rows, of a stage
 constexpr int STAGE_BYTES = 2 * HALF_BYTES;
-constexpr int STAGES = 6;
+constexpr int STAGES = 4;
 constexpr int kFoldWarps = 8;
 constexpr int kThreads = (kFoldWarps + 4) * 32;
 constexpr int kFoldRegs = 216, kOtherRegs = 72;   // together the launch's 384 x 168
@@ -45,9 +50,12 @@ constexpr int BAR_BYTES = 512;
 constexpr int SUM_PITCH = 260;                    // floats from token to token: 16-byte accesses of eight lanes take all banks
 constexpr int kMaxSplit = kMaxPairSplit;
 constexpr int AMAX_FLOATS = 2 * 2 * 128;          // [tile parity][column half][token]
-constexpr int STRIP_PITCH = 80;                    // bytes from token to token of a fold warp's strip: 64 and a shift of banks
+constexpr int OUT_BOX = 32 * 128;                  // 32 tokens x 64 channels on their way out, rows of 128 bytes swizzled as TMA has them
+constexpr int OUT_BYTES = kFoldWarps * 2 * OUT_BOX;
+constexpr int STRIP_PITCH = 80;                    // gated: bytes from token to token of a fold warp's strip: 64 and a shift of banks
 constexpr int STRIP_BYTES = 32 * STRIP_PITCH;
-constexpr int kSmemBytes = STAGES * STAGE_BYTES + BAR_BYTES + (kSlots * SLOT_FLOATS + AMAX_FLOATS) * 4 + kFoldWarps * STRIP_BYTES;
+constexpr int kSmemBytes = STAGES * STAGE_BYTES + OUT_BYTES + BAR_BYTES + (kSlots * SLOT_FLOATS + AMAX_FLOATS) * 4;
+static_assert(128 * SUM_PITCH * 4 <= STAGES * STAGE_BYTES + OUT_BYTES && STRIP_BYTES <= 2 * OUT_BOX, "sums, strips");
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 
 struct KernelParams {
@@ -90,9 +98,12 @@ struct Tile {
 // SPLIT: a tile per cluster of `split` pairs, each with a part of its K blocks
 template <bool GATED, bool MOVE, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
-fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const KernelParams p) {
+fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                       const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_addend, const KernelParams p) {
+  constexpr bool BOXES = !GATED && !SPLIT;  // the output leaves by TMA
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint8_t* outgoing = smem + STAGES * STAGE_BYTES;  // [fold warp][64 channels][token]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(outgoing + OUT_BYTES);
   uint64_t* full_bar = bars;                // [STAGES] used in CTA 0: both CTAs' loads -> MMA
   uint64_t* empty_bar = bars + STAGES;      // [STAGES] per CTA: MMA -> TMA
   uint64_t* part_full = bars + 2 * STAGES;  // [4] per CTA: MMA -> fold; 2 * (K block % 2) + half
@@ -100,10 +111,11 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
   uint64_t* sc_full = part_empty + 4;       // [kSlots]
   uint64_t* sc_empty = sc_full + kSlots;    // [kSlots]
   uint64_t* amax_bar = sc_empty + kSlots;   // [4] the two warps that hold a token's 128 channels
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(amax_bar + 4);
-  float* scales = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES + BAR_BYTES);
+  uint64_t* out_ready = amax_bar + 4;       // [1] the boxes are free, and hold the tile's addend
+  uint64_t* out_full = out_ready + 1;       // [kFoldWarps] a warp's boxes are complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(out_full + kFoldWarps);
+  float* scales = reinterpret_cast<float*>(outgoing + OUT_BYTES + BAR_BYTES);
   float* amax_buf = scales + kSlots * SLOT_FLOATS;
-  uint8_t* strips = reinterpret_cast<uint8_t*>(amax_buf + AMAX_FLOATS);
 
   const int warp = ptx::uniform_warp_id(), lane = threadIdx.x & 31;
   const int cluster_rank = (int)ptx::cluster_ctarank(), rank = cluster_rank & 1;
@@ -126,11 +138,14 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       ptx::mbar_init(&sc_empty[s], kFoldWarps);
     }
     for (int q = 0; q < 4; ++q) ptx::mbar_init(&amax_bar[q], 2);
+    ptx::mbar_init(out_ready, 1);
+    for (int q = 0; q < kFoldWarps; ++q) ptx::mbar_init(&out_full[q], 1);
     ptx::fence_barrier_init();
   }
   if (warp == kFoldWarps && lane == 0) {
     ptx::prefetch_tensormap(&map_x);
     ptx::prefetch_tensormap(&map_w);
+    if (BOXES) ptx::prefetch_tensormap(&map_out);
   }
   if (warp == kFoldWarps + 2) {
     ptx::tmem_alloc_pair(tmem_slot, 512);
@@ -221,16 +236,14 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         sc_step += kGroup - sc_step % kGroup;
       }
 
-      // The warp's 32 tokens leave through its strip, 64 bytes of each at a time: lane l holds token l's values, and stores those of
-      // tokens l / 4 + 8 i, 16 bytes each.  (Straight from the registers, 16 bytes per token and instruction, with the addend's loads
-      // one behind the other: 10 us per tile.)
-      const int64_t t0 = (int64_t)tl.token * 256 + rank * 128 + quarter * 32;
-      uint8_t* strip = strips + warp * STRIP_BYTES;
-      uint4* own = reinterpret_cast<uint4*>(strip + lane * STRIP_PITCH);
-      uint4* dealt = reinterpret_cast<uint4*>(strip + (lane >> 2) * STRIP_PITCH + (lane & 3) * 16);  // token lane / 4 + 8 i: 8 i rows on
-      constexpr int kDealtStep = 8 * STRIP_PITCH / 16;
-      const int mine = (int)min((int64_t)32, p.T - t0) - (lane >> 2);  // of the four tokens, those with 8 i < mine are there
       if constexpr (GATED) {
+        // The warp's 32 tokens leave through its strip: lane l holds token l's values, and stores those of tokens l / 4 + 8 i, 16 bytes each.
+        const int64_t t0 = (int64_t)tl.token * 256 + rank * 128 + quarter * 32;
+        uint8_t* strip = outgoing + warp * STRIP_BYTES;
+        uint4* own = reinterpret_cast<uint4*>(strip + lane * STRIP_PITCH);
+        uint4* dealt = reinterpret_cast<uint4*>(strip + (lane >> 2) * STRIP_PITCH + (lane & 3) * 16);  // token lane / 4 + 8 i: 8 i rows on
+        constexpr int kDealtStep = 8 * STRIP_PITCH / 16;
+        const int mine = (int)min((int64_t)32, p.T - t0) - (lane >> 2);  // of the four tokens, those with 8 i < mine are there
         float amax = 0.f;
         auto activate = [&](auto activation) {
 #pragma unroll
@@ -270,75 +283,63 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
           if (8 * i < mine) *reinterpret_cast<uint4*>(dst + 8 * i * p.n) = dealt[i * kDealtStep];
         __syncwarp();
       } else {
-        const int64_t ch0 = (int64_t)tl.w * 256 + piece * 128;
-        const int64_t at = (t0 + (lane >> 2)) * p.n + ch0 + (lane & 3) * 8;
-        const int cols = (int)min((int64_t)128, p.n - ch0);  // a multiple of 8, or nothing
-        uint4 more[4];
-        auto fetch = [&](int c) {  // the addend of 32 channels, as this lane will store them
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (8 * i < mine && c + (lane & 3) * 8 < cols) more[i] = *reinterpret_cast<const uint4*>(p.addend + at + 8 * i * p.n + c);
-        };
-        if (p.addend) fetch(0);
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) {
-          if (c < cols) {
-            if (p.bias) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                if (c + j < cols) {
-                  const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + ch0 + c + j));
-                  acc[c + j] += b.x;
-                  acc[c + j + 1] += b.y;
-                  acc[c + j + 2] += b.z;
-                  acc[c + j + 3] += b.w;
-                }
-              }
-            }
-            if (p.addend) {  // to the lanes that hold the sums: they are added before the one rounding
-#pragma unroll
-              for (int i = 0; i < 4; ++i) dealt[i * kDealtStep] = more[i];
-              if (c + 32 < cols) fetch(c + 32);
-              __syncwarp();
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const uint4 raw = own[q];
-                const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                  acc[c + 8 * q + 2 * u] += __low2float(e[u]);
-                  acc[c + 8 * q + 2 * u + 1] += __high2float(e[u]);
-                }
-              }
-              // a lane's own row: nobody else reads it before the next barrier
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float* v = acc + c + 8 * q;
-              own[q] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-            }
-            __syncwarp();
-            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + at + c;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (8 * i < mine && c + (lane & 3) * 8 < cols) *reinterpret_cast<uint4*>(dst + 8 * i * p.n) = dealt[i * kDealtStep];
-            __syncwarp();
-          }
+        // Into the warp's two boxes, which hold the addend's values so far, and on by TMA: the stores run beside the next tile.
+        if (!warp_wait(out_ready, ltile & 1)) {
+          report(0x2500);
+          break;
         }
+        const int64_t ch0 = (int64_t)tl.w * 256 + piece * 128;
+        uint8_t* row = outgoing + warp * 2 * OUT_BOX + lane * 128;
+#pragma unroll
+        for (int c = 0; c < 128; c += 8) {
+          uint4* at = reinterpret_cast<uint4*>(row + c / 64 * OUT_BOX + ((c / 8 % 8 ^ (lane & 7)) << 4));
+          if (p.bias && ch0 + c < p.n) {
+            const float4 b0 = __ldg(reinterpret_cast<const float4*>(p.bias + ch0 + c)), b1 = __ldg(reinterpret_cast<const float4*>(p.bias + ch0 + c) + 1);
+            acc[c] += b0.x;
+            acc[c + 1] += b0.y;
+            acc[c + 2] += b0.z;
+            acc[c + 3] += b0.w;
+            acc[c + 4] += b1.x;
+            acc[c + 5] += b1.y;
+            acc[c + 6] += b1.z;
+            acc[c + 7] += b1.w;
+          }
+          if (p.addend) {
+            const uint4 raw = *at;
+            const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              acc[c + 2 * u] += __low2float(e[u]);
+              acc[c + 2 * u + 1] += __high2float(e[u]);
+            }
+          }
+          *at = make_uint4(pack_bf16x2(acc[c], acc[c + 1]), pack_bf16x2(acc[c + 2], acc[c + 3]), pack_bf16x2(acc[c + 4], acc[c + 5]),
+                           pack_bf16x2(acc[c + 6], acc[c + 7]));
+        }
+        ptx::fence_proxy_async();
+        __syncwarp();
+        ptx::mbar_arrive_if(lane == 0, &out_full[warp]);
       }
     }
-  } else if (warp < kFoldWarps + 2) {
-    // ---------------- TMA: warp 8 its half of the tile's tokens, warp 9 its 128 weight rows ----------------
-    const bool weights = warp == kFoldWarps + 1;
+  } else if (warp == kFoldWarps) {
+    // ---------------- TMA: this CTA's half of the tile's tokens, and its 128 weight rows ----------------
     if (ptx::elect_one()) {
       const uint32_t ring = ptx::smem_u32(smem), bar_full0 = ptx::smem_u32(full_bar) & ~ptx::kPeerRankBit;
-      int stage = 0;
+      auto load_weights = [&](const Tile& tl, int kb, int s) {
+        // 64 rows for each half: 64 channels from here, or the same 64 channels' gate rows (CTA 0) and up rows
+        const int row = GATED ? tl.w * 128 + rank * (int)p.n : tl.w * 256 + rank * 64;
+        const uint32_t bar = bar_full0 + s * 8, dst = ring + s * STAGE_BYTES + HALF_BYTES;
+        ptx::tma_load_2d_pair(dst, &map_w, kb * KBYTES, row, bar);
+        ptx::tma_load_2d_pair(dst + HALF_BYTES / 2, &map_w, kb * KBYTES, row + (GATED ? 64 : 128), bar);
+      };
+      int stage = 0, ahead = 0;
       uint32_t phase = 0;
-      bool alive = true, waited = false;
-      if (!weights || !p.early) {
-        pdl_wait();
-        waited = true;
+      bool alive = true;
+      if (p.early) {  // weights that nothing before this kernel writes are on their way before the tokens are there
+        const Tile tl(worker, p);
+        for (ahead = 0; ahead < min(STAGES, kb1 - kb0); ++ahead) load_weights(tl, kb0 + ahead, ahead);
       }
+      pdl_wait();
       pdl_trigger();
       for (int i = worker; i < tiles && alive; i += workers) {
         const Tile tl(i, p);
@@ -348,16 +349,10 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             alive = false;
             break;
           }
-          const uint32_t bar = bar_full0 + stage * 8, dst = ring + stage * STAGE_BYTES;
-          if (weights) {
-            // 64 rows for each half: 64 channels from here, or the same 64 channels' gate rows (CTA 0) and up rows
-            const int row = GATED ? tl.w * 128 + rank * (int)p.n : tl.w * 256 + rank * 64;
-            ptx::tma_load_2d_pair(dst + HALF_BYTES, &map_w, kb * KBYTES, row, bar);
-            ptx::tma_load_2d_pair(dst + HALF_BYTES + HALF_BYTES / 2, &map_w, kb * KBYTES, row + (GATED ? 64 : 128), bar);
-          } else {
-            if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
-            ptx::tma_load_2d_pair(dst, &map_x, kb * KBYTES, tl.token * 256 + rank * 128, bar);
-          }
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+          ptx::tma_load_2d_pair(ring + stage * STAGE_BYTES, &map_x, kb * KBYTES, tl.token * 256 + rank * 128, bar_full0 + stage * 8);
+          if (ahead > 0) --ahead;
+          else load_weights(tl, kb, stage);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -374,7 +369,43 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
           phase ^= 1;
         }
       }
-      if (!waited) pdl_wait();
+    }
+    __syncwarp();
+  } else if (warp == kFoldWarps + 1) {
+    // ---------------- addend and output of a tile, by TMA ----------------
+    if (BOXES && ptx::elect_one()) {
+      pdl_wait();
+      const uint32_t boxes = ptx::smem_u32(outgoing);
+      bool alive = true;
+      int ltile = 0;
+      for (int i = worker; i < tiles && alive; i += workers, ++ltile) {
+        const Tile tl(i, p);
+        const int t0 = tl.token * 256 + rank * 128, ch0 = tl.w * 256;
+        const int quarters = p.T > t0 ? min(4, (p.T - t0 + 31) / 32) : 0, cols = (int)min((int64_t)4, (p.n - ch0 + 63) / 64);
+        auto box = [&](int quarter, int c) { return boxes + ((c >> 1) * 8 + quarter * 2 + (c & 1)) * OUT_BOX; };
+        ptx::tma_store_wait_read();
+        if (p.addend) {
+          ptx::mbar_arrive_expect_tx(out_ready, quarters * cols * OUT_BOX);
+          for (int c = 0; c < cols; ++c)
+            for (int q = 0; q < quarters; ++q) ptx::tma_load_2d(box(q, c), &map_addend, ch0 + 64 * c, t0 + 32 * q, ptx::smem_u32(out_ready));
+        } else {
+          ptx::mbar_arrive(out_ready);
+        }
+        if (!ptx::mbar_wait(out_ready, ltile & 1)) {  // and nothing is in flight when this CTA ends
+          report(0x2540);
+          break;
+        }
+        for (int w = 0; w < kFoldWarps && alive; ++w) {
+          if (!ptx::mbar_wait_relaxed(&out_full[w], ltile & 1)) {
+            report(0x2580 | w);
+            alive = false;
+          } else if ((w & 3) < quarters) {
+            for (int c = w / 4 * 2; c < min(cols, w / 4 * 2 + 2); ++c) ptx::tma_store_2d(&map_out, box(w & 3, c), ch0 + 64 * c, t0 + 32 * (w & 3));
+          }
+        }
+        ptx::tma_store_commit();
+      }
+      ptx::tma_store_wait();
     }
     __syncwarp();
   } else if (warp == kFoldWarps + 2) {
@@ -430,7 +461,7 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       const int t0 = tl.token * 256 + rank * 128 + lane;
       const int b0 = GATED ? tl.w : 2 * tl.w, b1 = GATED ? tl.w + (int)(p.n / 128) : min(2 * tl.w + 1, p.w_blocks - 1);
       const float* w_mine = p.w_scale + (int64_t)(lane & 1 ? b1 : b0) * p.kblocks;  // lanes 0-15: K block lane / 2, block lane % 2
-      if (!GATED && p.addend) {  // on its way to L2 while the tile is multiplied: all workers read theirs at about the same time
+      if (!GATED && SPLIT && p.addend) {  // on its way to L2 while the tile is multiplied: all workers read theirs at about the same time
         const int64_t t = tl.token * 256 + rank * 128, ch = (int64_t)tl.w * 256;
         const int lines = (int)(min((int64_t)256, p.n - ch) * 2 + 127) / 128;
         for (int r = lane; r < 128 && t + r < p.T; r += 32)
@@ -558,7 +589,16 @@ int launch(const LinearParams& g, int split, cudaStream_t st) {
   const int64_t tiles = (int64_t)p.token_tiles * p.w_tiles;
   const int sms = device_sm_count();
   const int workers = (int)(SPLIT ? tiles : std::min<int64_t>((sms > 0 ? sms : 148) / 2, tiles));
-  launch_pdl_cluster(kernel, 2 * split, dim3(2 * split * workers), dim3(kThreads), kSmemBytes, st, map_x, map_w, p);
+  CUtensorMap map_out = {}, map_addend = {};
+  if (!GATED && !SPLIT) {
+    const cuuint64_t out_dims[2] = {(cuuint64_t)g.n, (cuuint64_t)g.T};
+    const cuuint64_t out_strides[1] = {(cuuint64_t)g.n * 2};
+    const cuuint32_t out_box[2] = {64, 32};
+    rc = encode_tensor_map(&map_out, g.out, 2, 2, out_dims, out_strides, out_box, false, "output");
+    if (!rc && g.addend) rc = encode_tensor_map(&map_addend, g.addend, 2, 2, out_dims, out_strides, out_box, false, "addend");
+    if (rc) return rc;
+  }
+  launch_pdl_cluster(kernel, 2 * split, dim3(2 * split * workers), dim3(kThreads), kSmemBytes, st, map_x, map_w, map_out, map_addend, p);
   return launch_status("fp8_linear_pair_kernel");
 }
 
