@@ -4,7 +4,9 @@
 // (quotients: rows.cuh)
 // A CTA owns a row at a time and keeps it in registers between the sum of squares and the outputs, so every byte is read and
 // written once: HBM bounds it from some ten MB on (beside the issue slots, where a row has neither residual nor norm to move), the
-// launch and the dependent reductions below that: one row of 7168 takes 3 us.
+// launch and the dependent reductions below that: one row of 7168 takes 3 us.  Rows of which only the quantised norm is wanted run at 0.4
+// to 0.55 of the copy rate (8192 rows of 7168 bf16 62 us): 26 instructions per value, 70 % of the issue slots.  Two values per instruction
+// (f32x2), four vectors per thread instead of two, or no bounds predicates change that by 5 % at most, and cost rows with a residual as much.
 #include <algorithm>
 #include <type_traits>
 
