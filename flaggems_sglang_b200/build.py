@@ -65,7 +65,7 @@ def _host_command() -> list[str]:
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DBUILT_FOR_TORCH="{torch.__version__}"',
             "-I", sysconfig.get_paths()["include"], "-I", os.path.join(base, "include"),
             "-I", os.path.join(base, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
-            HOST_SRC, "-o", HOST_PATH, "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
+            HOST_SRC, "-o", HOST_PATH, "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lc10", "-lc10_cuda"]
 
 
 def ptxas_report(src: str) -> str:

@@ -5,7 +5,9 @@
 // it (17 for the MLP), of which the launch is 2.
 #include <Python.h>
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -34,8 +36,10 @@ bool is(const at::Tensor* t, c10::Device device, at::ScalarType type, int64_t ro
   return is(t, device, type, 2) && t->size(0) == rows && t->size(1) == cols;
 }
 
+// past the dispatcher, where no mode wants to see the call
 at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
-  return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
+  if (c10::impl::dispatch_mode_enabled()) return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
+  return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
 
 int code_of(at::ScalarType t) { return t == at::kBFloat16 ? FMOE_BF16 : (t == at::kFloat ? FMOE_F32 : -1); }
