@@ -5,7 +5,7 @@
 // A CTA owns a row at a time and keeps it in registers between the sum of squares and the outputs, so every byte is read and
 // written once: HBM bounds it from some ten MB on (beside the issue slots, where a row has neither residual nor norm to move), the
 // launch and the dependent reductions below that: one row of 7168 takes 3 us.  Rows of which only the quantised norm is wanted run at 0.4
-// to 0.55 of the copy rate (8192 rows of 7168 bf16 62 us): 26 instructions per value, 70 % of the issue slots.  Two values per instruction
+// to 0.6 of the copy rate (8192 rows of 7168 bf16 58 us): 26 instructions per value, 70 % of the issue slots.  Two values per instruction
 // (f32x2), four vectors per thread instead of two, or no bounds predicates change that by 5 % at most, and cost rows with a residual as much.
 #include <algorithm>
 #include <type_traits>
@@ -151,16 +151,16 @@ __device__ __forceinline__ void add_residual(const NormParams& p, T* res, float 
   }
 }
 
-// Few rows: a CTA per row, loads straight into registers.
-template <typename T, int VECS, bool PER_TOKEN>
-__global__ void __launch_bounds__(1024)
+// A CTA per row, loads straight into registers.  MAX_THREADS 448: three CTAs of so many threads on an SM (40 registers).
+template <typename T, int VECS, bool PER_TOKEN, bool RESIDUAL, int MAX_THREADS>
+__global__ void __launch_bounds__(MAX_THREADS, MAX_THREADS == 448 ? 3 : 1)
 rms_norm_quant_kernel(const NormParams p) {
   pdl_entry_late();
   __shared__ float buf[2][32];
   const int vecs = p.K / 8;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.x_stride;
-    T* res = p.residual ? reinterpret_cast<T*>(p.residual) + row * p.residual_stride : nullptr;
+    T* res = RESIDUAL ? reinterpret_cast<T*>(p.residual) + row * p.residual_stride : nullptr;
     float h[VECS][8], r[VECS][8];
     // every load of the row is on its way before the first sum is stored
 #pragma unroll
@@ -170,19 +170,17 @@ rms_norm_quant_kernel(const NormParams p) {
       for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
       if (c < vecs) {
         load8(x + 8 * c, h[i]);
-        if (res) load8(res + 8 * c, r[i]);
+        if constexpr (RESIDUAL) load8(res + 8 * c, r[i]);
       }
     }
-    if (res) add_residual<T, VECS>(p, res, h, r);
+    if constexpr (RESIDUAL) add_residual<T, VECS>(p, res, h, r);
     finish_row<T, VECS, PER_TOKEN>(p, row, h, buf, true);
   }
 }
 
-// Many bf16 rows: persistent CTAs whose rows arrive in a ring of shared memory (one bulk copy per row and tensor), so that the next
-// rows' bytes are on their way while this one is reduced.  8192 rows of 7168 with residual and norm: 135 us with loads into registers
-// (two CTAs of 448 threads fit an SM, 57 KB on their way), 90 us here, 5.9 TB/s.  Rows of fp32 have twice the bytes per thread and do
-// better without the detour: 4096 rows of 8192 90 us (5.8 TB/s) against 104.  Four 16-byte pieces per thread instead of two spread the
-// reductions over more values but leave fewer warps: 93 us.
+// Long bf16 rows: persistent CTAs whose rows arrive in a ring of shared memory (one bulk copy per row and tensor), so that the next
+// rows' bytes are on their way while this one is reduced.  With residual and norm 8192 rows of 7168 take 98 us with loads into registers (two
+// CTAs of 448 threads fit an SM), 90 us here, 5.9 TB/s; of 6144, where three CTAs fit, 74 and 79, of 2944 37 and 42.
 template <bool PER_TOKEN, int MAX_THREADS>
 __global__ void __launch_bounds__(MAX_THREADS, MAX_THREADS > 512 ? 1 : 3)
 rms_norm_quant_stream_kernel(const NormParams p, int stages) {
@@ -301,7 +299,10 @@ extern "C" int fmoe_rms_norm_quant(const void* x, int64_t x_stride, void* residu
     if (dtype == FMOE_BF16) per_token ? go((__nv_bfloat16*)nullptr, std::true_type{}) : go((__nv_bfloat16*)nullptr, std::false_type{});
     else per_token ? go((float*)nullptr, std::true_type{}) : go((float*)nullptr, std::false_type{});
   };
-  if (dtype == FMOE_BF16 && rows > 296) {  // 400 rows of 7168: 6.3 us, in registers 7.9; 77 rows 3.9 and 3.7
+  // Many rows (us of 8192 without residual; in registers, there with three CTAs of up to 448 threads, by the ring): bf16 4096 channels 34.5,
+  // 31.2, 37.1, 7168 67.8, 58.3, 61.6; fp32 4096 36.0, 37.4, 7168 76.2, 68.8.  With residual that many registers do not do.
+  const bool many = rows > 296, three = many && !residual && threads(2) <= 448 && (dtype == FMOE_BF16 || threads(2) > 256);
+  if (dtype == FMOE_BF16 && many && !three && (!residual || threads(2) > 384)) {
     const int stage_bytes = (int)K * 2 * (residual ? 2 : 1);
     const int ctas = std::min(std::max(1, 1536 / (int)threads(2)), (kStreamBytes - 2048) / (2 * stage_bytes + 1024));  // at least 1: K <= 16384
     const int stages = std::min(kMaxStages, (kStreamBytes / ctas - 1024) / stage_bytes);
@@ -328,9 +329,13 @@ extern "C" int fmoe_rms_norm_quant(const void* x, int64_t x_stride, void* residu
     using E = std::remove_pointer_t<decltype(type)>;
     auto with = [&](auto v) {
       constexpr int VV = decltype(v)::value;
-      launch_pdl(rms_norm_quant_kernel<E, VV, decltype(token)::value>, dim3((unsigned)std::min<int64_t>(rows, 148 * 32)), dim3(threads(VV)), 0, st, p);
+      constexpr bool PER_TOKEN = decltype(token)::value;
+      auto kernel = residual ? rms_norm_quant_kernel<E, VV, PER_TOKEN, true, 1024> : rms_norm_quant_kernel<E, VV, PER_TOKEN, false, 1024>;
+      if constexpr (VV == 2)
+        if (three) kernel = rms_norm_quant_kernel<E, 2, PER_TOKEN, false, 448>;
+      launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(rows, 148 * 32)), dim3(threads(VV)), 0, st, p);
     };
-    if (vecs <= 1024 && rows <= 296) with(std::integral_constant<int, 1>{});
+    if (vecs <= 1024 && !many) with(std::integral_constant<int, 1>{});
     else with(std::integral_constant<int, 2>{});
   });
   return launch_status("rms_norm_quant_kernel");
