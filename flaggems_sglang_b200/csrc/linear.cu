@@ -13,7 +13,8 @@
 //             fill the chip.  Their sums meet through distributed shared memory, added in the order of the CTAs: the result does not
 //             depend on timing, and there is no scratch in global memory and no counter.  Up to 64 tokens every CTA sends its sums to the
 //             ones that store them (st.async, one mbarrier there; against two cluster barriers and reading the others' memory one token
-//             of 7168 x 2048 4.7 -> 4.2 us, 16 tokens of 2048 x 7168 5.1 -> 4.2); 128 tokens have no room to land
+//             of 7168 x 2048 4.7 -> 4.2 us, 16 tokens of 2048 x 7168 5.1 -> 4.2); tiles of 128 tokens keep theirs, which
+//             the others read (sent, 128 tokens of 2048 x 7168 took 8.4 us against 7.5)
 //   warps   : fold warps (TMEM lane quarter = warp % 4; 16 or 32 sums per thread), then TMA, MMA, and two that multiply token and weight
 //             scales into a ring of factors
 //   batches : up to 32 tokens the partials of two or four K blocks are handed to the fold together.  What a K block costs there is not
@@ -27,7 +28,7 @@
 // or gate and up rows in one CTA bring, makes the fold take twice as long: 64 tokens 38 us for 56 K blocks against 17.7 with one CTA.)
 // Every mbarrier wait is bounded; the cluster barriers are reached by every thread on every path.
 // What bounds it: up to 64 tokens HBM beside the launch, the first loads and the join (one token, 7168 x 4096: 6.2 us, 4.7 TB/s; gate/up of
-// 7168 x 2 x 2048 7.1 us); with 128 tokens shared memory, 32 KB in and 32 KB of operands per K block (0.27 us).
+// 7168 x 2 x 2048 6.6 us); with 128 tokens shared memory, 32 KB in and 32 KB of operands per K block (0.27 us).
 #include "linear.cuh"
 #include "pair.cuh"
 #include "rows.cuh"

@@ -54,9 +54,12 @@ constexpr int OUT_BOX = 32 * 128;                  // 32 tokens x 64 channels on
 constexpr int OUT_BYTES = kFoldWarps * 2 * OUT_BOX;
 constexpr int STRIP_PITCH = 80;                    // gated: bytes from token to token of a fold warp's strip: 64 and a shift of banks
 constexpr int STRIP_BYTES = 32 * STRIP_PITCH;
-constexpr int kSmemBytes = STAGES * STAGE_BYTES + OUT_BYTES + BAR_BYTES + (kSlots * SLOT_FLOATS + AMAX_FLOATS) * 4;
+constexpr int kSmemUsed = STAGES * STAGE_BYTES + OUT_BYTES + BAR_BYTES + (kSlots * SLOT_FLOATS + AMAX_FLOATS) * 4;
+// All of an SM's: a CTA of another kernel that fitted beside and had TMEM would wait here for this one's end (512 columns), while its cluster
+// waits for it, or this one for that one's.
+constexpr int kSmemBytes = 227 * 1024;
+static_assert(kSmemUsed <= kSmemBytes, "shared memory");
 static_assert(128 * SUM_PITCH * 4 <= STAGES * STAGE_BYTES + OUT_BYTES && STRIP_BYTES <= 2 * OUT_BOX, "sums, strips");
-static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 
 struct KernelParams {
   const float* x_scale;

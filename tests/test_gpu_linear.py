@@ -461,3 +461,37 @@ def test_rows_of_nan_are_quantised_as_by_the_quantiser():
     assert torch.isnan(got[3]).all()
     keep = [t for t in range(70) if t != 3]
     assert torch.equal(got[keep], want[keep])
+
+
+def test_many_and_few_tokens_at_once():
+    """Captured calls of every kind (rows quantised in the product, shared tiles, pairs with an addend) replayed on three streams at a time."""
+    K, I, N = 1024, 512, 2048
+    w13, s13 = weight(2 * I, K, 91)
+    w2, s2 = weight(N, I, 92)
+    w, ws = weight(N, K, 93)
+    calls = []
+    for i, T in enumerate((3, 100, 2500)):
+        x = rows(T, K, 94 + i, wide=False).bfloat16()
+        addend = torch.randn(T, N, generator=gen(97 + i), device="cuda").bfloat16()
+
+        def call(x=x, addend=addend):
+            return fg().fp8_gated_mlp(x, w13, s13, w2, s2, addend=fg().fp8_block_linear(x, w, ws, addend=addend))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = call().clone()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = call()
+        calls.append((g, y, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, _, _, s in calls:
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for _, y, want, _ in calls:
+        assert torch.equal(y, want)
+    status()
