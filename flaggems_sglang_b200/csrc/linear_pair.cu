@@ -414,6 +414,7 @@ fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
   } else if (warp == kFoldWarps + 2) {
     // ---------------- MMA issuer (CTA 0): one fresh partial per K block ----------------
     if (rank == 0 && ptx::elect_one()) {
+      pdl_wait();  // the limit of the waits below counts from here: a kernel ahead of this one may run on for any time
       const uint32_t ring = ptx::smem_u32(smem);
       const uint64_t da0 = ptx::smem_desc_sw128(ring), db0 = ptx::smem_desc_sw128(ring + HALF_BYTES);
       constexpr uint32_t idesc = ptx::make_idesc(/*e4m3*/ 0, 256, 128);
