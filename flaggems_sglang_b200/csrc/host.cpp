@@ -36,6 +36,13 @@ bool is(const at::Tensor* t, c10::Device device, at::ScalarType type, int64_t ro
   return is(t, device, type, 2) && t->size(0) == rows && t->size(1) == cols;
 }
 
+// Other Python threads run meanwhile: allocations and launches may wait (for memory, for room in the stream's queue), perhaps for what
+// another thread has yet to launch.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 // past the dispatcher, where no mode wants to see the call
 at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
   if (c10::impl::dispatch_mode_enabled()) return at::empty(sizes, at::TensorOptions().dtype(type).device(device));
@@ -94,16 +101,22 @@ PyObject* finish(Operands& o, PyObject* addend, Run run, Bytes bytes) {
     if (!is(o.addend, dev, at::kBFloat16, o.a.T, o.a.N)) Py_RETURN_NONE;
     o.a.addend = o.addend->const_data_ptr();
   }
-  at::Tensor out = make({o.a.T, o.a.N}, at::kBFloat16, dev), ws;
-  o.a.out = out.mutable_data_ptr();
-  const int64_t need = bytes(&o.a);
-  if (need < 0) Py_RETURN_NONE;  // the Python function says why
-  if (need > 0) {
-    ws = make({need}, at::kByte, dev);
-    o.a.workspace = ws.mutable_data_ptr();
-    o.a.workspace_bytes = need;
+  at::Tensor out, ws;
+  int64_t need;
+  int rc = FMOE_OK;
+  {
+    Unlocked other_threads_run;
+    out = make({o.a.T, o.a.N}, at::kBFloat16, dev);
+    o.a.out = out.mutable_data_ptr();
+    need = bytes(&o.a);
+    if (need > 0) {
+      ws = make({need}, at::kByte, dev);
+      o.a.workspace = ws.mutable_data_ptr();
+      o.a.workspace_bytes = need;
+    }
+    if (need >= 0) rc = run(&o.a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   }
-  const int rc = run(&o.a, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  if (need < 0) Py_RETURN_NONE;  // the Python function says why
   if (rc != FMOE_OK) return PyLong_FromLong(rc);
   return THPVariable_Wrap(std::move(out));
 }
@@ -158,13 +171,20 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t rows = x->size(0), K = x->size(1);
   if (rows == 0 || K == 0 || K > 16384 || K % (per_token ? 8 : 128) || weight->size(0) != K) Py_RETURN_NONE;
   if (residual && !is(residual, dev, type, rows, K)) Py_RETURN_NONE;
-  at::Tensor q = make({rows, K}, kE4M3, dev), out;
-  at::Tensor s = per_token ? make({rows}, at::kFloat, dev) : make({rows, K / 128}, at::kFloat, dev);
-  if (keep) out = make({rows, K}, type, dev);
-  const int rc = entry.norm(x->const_data_ptr(), K, residual ? residual->mutable_data_ptr() : nullptr, K, code, weight->const_data_ptr(), w_code,
-                            rows, K, (float)PyFloat_AS_DOUBLE(args[2]), per_token, q.mutable_data_ptr(),
-                            static_cast<float*>(s.mutable_data_ptr()), keep ? out.mutable_data_ptr() : nullptr,
-                            c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  const void *x_data = x->const_data_ptr(), *weight_data = weight->const_data_ptr();
+  void* residual_data = residual ? residual->mutable_data_ptr() : nullptr;
+  const float eps = (float)PyFloat_AS_DOUBLE(args[2]);
+  at::Tensor q, s, out;
+  int rc;
+  {
+    Unlocked other_threads_run;
+    q = make({rows, K}, kE4M3, dev);
+    s = per_token ? make({rows}, at::kFloat, dev) : make({rows, K / 128}, at::kFloat, dev);
+    if (keep) out = make({rows, K}, type, dev);
+    rc = entry.norm(x_data, K, residual_data, K, code, weight_data, w_code, rows, K, eps, per_token, q.mutable_data_ptr(),
+                    static_cast<float*>(s.mutable_data_ptr()), keep ? out.mutable_data_ptr() : nullptr,
+                    c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  }
   if (rc != FMOE_OK) return PyLong_FromLong(rc);
   PyObject* result = PyTuple_New(keep ? 3 : 2);
   if (!result) return nullptr;

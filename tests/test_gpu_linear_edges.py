@@ -43,3 +43,52 @@ def test_limit_of_the_waits_does_not_count_the_kernel_before(early_trigger, kern
     got = fg().fp8_block_linear(xq, w, ws, x_scale=xs)
     status()
     assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
+def test_other_python_threads_run_while_a_call_waits_for_its_launch(tmp_path):
+    """A launch waits where the stream's queue is full, perhaps for what another thread has yet to launch: the interpreter is free meanwhile."""
+    import threading
+    import time
+
+    from flaggems_sglang_b200 import _C
+
+    host, cc = _C.host(), shutil.which("gcc")
+    if not cc:
+        pytest.skip("no gcc")
+    assert host, "the compiled module is not built"
+    src, so = tmp_path / "slow.c", tmp_path / "slow.so"
+    src.write_text("#include <time.h>\nint slow(void) { struct timespec t = {0, 500000000}; nanosleep(&t, 0); return 0; }\n"
+                   "long long none(void) { return 0; }\n")
+    subprocess.run([cc, "-shared", "-fPIC", str(src), "-o", str(so)], check=True)
+    lib = ctypes.CDLL(str(so))
+    slow, none = (ctypes.cast(f, ctypes.c_void_p).value for f in (lib.slow, lib.none))
+    w, ws = weight(256, 512, 3)
+    w13, s13 = weight(256, 512, 4)
+    w2, s2 = weight(512, 128, 5)
+    x = rows(4, 512, 6).bfloat16()
+    calls = [lambda: fg().fp8_block_linear(x, w, ws), lambda: fg().fp8_gated_mlp(x, w13, s13, w2, s2),
+             lambda: fg().rms_norm_quant_fp8(x, torch.ones(512, device="cuda"))]
+    for call in calls:
+        call()
+    ticks, done = [], threading.Event()
+
+    def tick():
+        while not done.wait(0.005):
+            ticks.append(time.perf_counter())
+
+    thread = threading.Thread(target=tick)
+    thread.start()
+    try:
+        host.bind(slow, slow, none, slow, none)
+        for call in calls:
+            t0 = time.perf_counter()
+            call()
+            t1 = time.perf_counter()
+            assert t1 - t0 > 0.45, "the call did not go through the module"
+            assert sum(t0 + 0.05 < t < t1 - 0.05 for t in ticks) > 5
+    finally:
+        done.set()
+        thread.join()
+        _C._host = None
+        _C.host()  # the library's entry points again
+    assert torch.isfinite(calls[0]()).all()
