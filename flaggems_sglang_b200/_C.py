@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import warnings
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_uint32, c_void_p
 
 import torch  # noqa: F401  (loads the CUDA runtime the library links against)
@@ -193,17 +194,21 @@ _host = None
 
 
 def host():
-    """The module of csrc/host.cpp, bound to the loaded library; False where it has not been built for this torch (the operators then
-    take the longer way, through ctypes, to the same entry points)."""
+    """The module of csrc/host.cpp, bound to the loaded library; False where it has not been built, or for another torch or Python (which
+    is said once): the operators then take the longer way, through ctypes, to the same entry points."""
     global _host
     if _host is None:
         handle = lib()
         try:
             from . import _host as module
-        except ImportError:
-            module = None
-        if module is None or module.torch_version != torch.__version__:
+            wrong = None if module.torch_version == torch.__version__ else f"it was built for torch {module.torch_version}"
+        except ImportError as e:
+            wrong = str(e) if os.path.exists(os.path.join(_HERE, "_host.so")) else ""
+        if wrong is not None:
             _host = False
+            if wrong:
+                warnings.warn(f"the compiled module beside the library is not used ({wrong}): build it with "
+                              "`python -m flaggems_sglang_b200.build`", RuntimeWarning, stacklevel=3)
         else:
             module.bind(*(ctypes.cast(getattr(handle, "fmoe_" + name), c_void_p).value for name in (
                 "rms_norm_quant", "fp8_linear", "fp8_linear_workspace_bytes", "fp8_mlp", "fp8_mlp_workspace_bytes")))

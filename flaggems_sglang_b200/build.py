@@ -4,8 +4,9 @@
 
 The library is a plain C-ABI shared object (see include/fmoe_b200.h); it links
 only the CUDA runtime.  Objects are rebuilt when a source or header is newer.
-Beside it _host.so is built from csrc/host.cpp, the short way from Python into some
-of the operators; it calls the library through the same C entry points.
+Behind it _host.so is built from csrc/host.cpp, the short way from Python into some
+of the operators; it calls the library through the same C entry points, and where it
+cannot be built (no C++ compiler, other torch headers) they are called through ctypes.
 """
 from __future__ import annotations
 
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -55,8 +57,6 @@ HOST_PATH = os.path.join(HERE, "_host.so")
 
 def _host_command() -> list[str]:
     """The module with the short way into some of the operators: C++ against the torch and Python of this interpreter."""
-    import sysconfig
-
     import torch
 
     base = os.path.dirname(torch.__file__)
@@ -66,6 +66,40 @@ def _host_command() -> list[str]:
             "-I", sysconfig.get_paths()["include"], "-I", os.path.join(base, "include"),
             "-I", os.path.join(base, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
             HOST_SRC, "-o", HOST_PATH, "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lc10", "-lc10_cuda"]
+
+
+def _build_host(force: bool, verbose: bool) -> None:
+    """_host.so, where the sources or the command (and with it torch or Python) are other than those it was built by."""
+    try:
+        cmd = _host_command()
+    except ImportError:
+        sys.stderr.write("no torch: csrc/host.cpp is not built\n")
+        return
+    words = " ".join(w for w in cmd if w not in (HOST_SRC, HOST_PATH))  # the tree may be elsewhere now
+    record = os.path.join(OBJ_DIR, "host.command")
+    built_by = open(record).read() if os.path.exists(record) else None
+    newest = max(os.path.getmtime(HOST_SRC), os.path.getmtime(os.path.join(INCLUDE, "fmoe_b200.h")))
+    if not force and built_by == words and os.path.exists(HOST_PATH) and os.path.getmtime(HOST_PATH) >= newest:
+        return
+    if os.path.exists(HOST_PATH):
+        os.remove(HOST_PATH)
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        why = "no Python.h"
+    else:
+        try:
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            why = None if r.returncode == 0 else " ".join(cmd) + "\n" + r.stdout + r.stderr
+        except OSError as e:
+            why = str(e)
+    if why is not None:
+        if os.path.exists(HOST_PATH):
+            os.remove(HOST_PATH)
+        sys.stderr.write(f"{why}\ncsrc/host.cpp is not built: its operators are called through ctypes\n")
+        return
+    if verbose:
+        sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+    with open(record, "w") as f:
+        f.write(words)
 
 
 def ptxas_report(src: str) -> str:
@@ -90,18 +124,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         return cmd, r
 
-    import sysconfig
-
-    host_stale = force or not os.path.exists(HOST_PATH) or os.path.getmtime(HOST_PATH) < max(
-        os.path.getmtime(HOST_SRC), os.path.getmtime(os.path.join(INCLUDE, "fmoe_b200.h")))
-    if host_stale and not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
-        sys.stderr.write("no Python.h: the operators of csrc/host.cpp are called through ctypes\n")
-    elif host_stale:
-        cmd, r = run(_host_command())
-        if verbose or r.returncode != 0:
-            sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
-        if r.returncode != 0:
-            raise RuntimeError("compilation of csrc/host.cpp failed")
     if jobs:
         with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
             for cmd, r in ex.map(run, jobs):
@@ -117,6 +139,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    _build_host(force, verbose)
     return LIB_PATH
 
 

@@ -5,6 +5,8 @@
 // it (17 for the MLP), of which the launch is 2.
 #include <Python.h>
 
+#include <cstring>
+
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -211,6 +213,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+#define TEXT_OF(x) #x
+#define TEXT(x) TEXT_OF(x)
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL
 PyMethodDef methods[] = {{"bind", FAST(bind), nullptr},
                          {"norm", FAST(norm), nullptr},
@@ -222,7 +226,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods};
 }  // namespace
 
 extern "C" __attribute__((visibility("default"))) PyObject* PyInit__host() {
-  if (Py_Version >> 16 != PY_VERSION_HEX >> 16) return PyErr_Format(PyExc_ImportError, "built for another version of Python");
+  constexpr char built[] = TEXT(PY_MAJOR_VERSION) "." TEXT(PY_MINOR_VERSION) ".";
+  if (strncmp(Py_GetVersion(), built, sizeof built - 1) != 0) return PyErr_Format(PyExc_ImportError, "built for another version of Python");
   PyObject* m = PyModule_Create(&module);
   if (m && PyModule_AddStringConstant(m, "torch_version", BUILT_FOR_TORCH) < 0) Py_CLEAR(m);
   return m;
