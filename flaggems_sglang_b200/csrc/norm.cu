@@ -181,8 +181,9 @@ rms_norm_quant_kernel(const NormParams p) {
 // Long bf16 rows: persistent CTAs whose rows arrive in a ring of shared memory (one bulk copy per row and tensor), so that the next
 // rows' bytes are on their way while this one is reduced.  With residual and norm 8192 rows of 7168 take 98 us with loads into registers (two
 // CTAs of 448 threads fit an SM), 90 us here, 5.9 TB/s; of 6144, where three CTAs fit, 74 and 79, of 2944 37 and 42.
+// MAX_THREADS 512, 768: three and two CTAs of so many threads on an SM (40 registers); 1024: one (52), or two of up to 576.
 template <bool PER_TOKEN, int MAX_THREADS>
-__global__ void __launch_bounds__(MAX_THREADS, MAX_THREADS > 512 ? 1 : 3)
+__global__ void __launch_bounds__(MAX_THREADS, 1536 / MAX_THREADS)
 rms_norm_quant_stream_kernel(const NormParams p, int stages) {
   using T = __nv_bfloat16;
   constexpr int VECS = 2;
@@ -304,6 +305,9 @@ extern "C" int fmoe_rms_norm_quant(const void* x, int64_t x_stride, void* residu
   const bool many = rows > 296, three = many && !residual && threads(2) <= 448 && (dtype == FMOE_BF16 || threads(2) > 256);
   if (dtype == FMOE_BF16 && many && !three && (!residual || threads(2) > 384)) {
     const int stage_bytes = (int)K * 2 * (residual ? 2 : 1);
+    // Above 576 threads two CTAs fit with 40 registers, not with 52: 8192 rows of 9728 with residual 118 us and 134, of 12288 150 and 153,
+    // without 82 and 95, 97 and 105; of 8704 (544 threads, two fit either way) 108 and 106, 77 and 72.  With a scale per row 40 registers
+    // spill (12288 with residual 161 and 153, 9728 132 and 133, without 88 and 94): the larger kernel, half of whose CTAs wait.
     const int ctas = std::min(std::max(1, 1536 / (int)threads(2)), (kStreamBytes - 2048) / (2 * stage_bytes + 1024));  // at least 1: K <= 16384
     const int stages = std::min(kMaxStages, (kStreamBytes / ctas - 1024) / stage_bytes);
     cudaError_t attr_err = cudaSuccess;
@@ -311,14 +315,18 @@ extern "C" int fmoe_rms_norm_quant(const void* x, int64_t x_stride, void* residu
       constexpr bool PER_TOKEN = decltype(token)::value;
       auto kernel = rms_norm_quant_stream_kernel<PER_TOKEN, 512>;
       auto wide = rms_norm_quant_stream_kernel<PER_TOKEN, 1024>;
+      auto middle = rms_norm_quant_stream_kernel<false, 768>;
       static PerDeviceOnce once_attr;
       attr_err = per_device_once(once_attr, [&] {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
-        return e != cudaSuccess ? e : cudaFuncSetAttribute(wide, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
+        cudaError_t e = cudaSuccess;
+        for (auto k : {kernel, middle, wide})
+          if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamBytes);
+        return e;
       });
       if (attr_err != cudaSuccess) return;
       const unsigned grid = (unsigned)std::min<int64_t>(rows, (int64_t)148 * ctas);
-      launch_pdl(threads(2) > 512 ? wide : kernel, dim3(grid), dim3(threads(2)), (size_t)stages * stage_bytes, st, p, stages);
+      const bool two = !PER_TOKEN && threads(2) > 576 && threads(2) <= 768;
+      launch_pdl(two ? middle : (threads(2) > 512 ? wide : kernel), dim3(grid), dim3(threads(2)), (size_t)stages * stage_bytes, st, p, stages);
     };
     if (per_token) go(std::true_type{});
     else go(std::false_type{});

@@ -115,3 +115,23 @@ def test_ops_refuse_cpu_tensors():
                  lambda: fg.fp8_gated_mlp(x, w, torch.ones(1, 2), w, torch.ones(1, 2))):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_norm_kernels_have_the_registers_that_their_plan_counts_on(C):
+    """CTAs an SM that the rows' ring is cut into: three of up to 512 threads, two of up to 576 and of up to 768, without a spill where rows
+    have a scale per 128 channels.  An SM has 65536 registers; a thread's are a multiple of eight."""
+    import re
+
+    from flaggems_sglang_b200.build import ptxas_report
+
+    found = {}
+    for name, spills, regs in re.findall(r"Compiling entry function '(\S+)'.*?(\d+) bytes spill stores.*?Used (\d+) registers",
+                                         open(ptxas_report("norm.cu")).read(), flags=re.S):
+        kernel = re.search(r"stream_kernelILb([01])ELi(\d+)E", name)
+        if kernel:
+            found[kernel[1] == "1", int(kernel[2])] = int(spills), -(-int(regs) // 8) * 8
+    assert set(found) == {(False, 512), (False, 768), (False, 1024), (True, 512), (True, 1024)}
+    for (per_token, most), (spills, regs) in found.items():
+        for threads, ctas in {512: ((512, 3),), 768: ((768, 2),), 1024: ((1024, 1), (576, 2))}[most]:
+            assert regs * threads * ctas <= 65536, (per_token, most, regs)
+        assert per_token or spills == 0
