@@ -51,10 +51,13 @@ __device__ __forceinline__ uint2 quant8(const float (&v)[8], float s, float r, b
 }
 
 // Division costs most of the instructions of a quantiser that is written with __fdiv_rn (the norm: 42 per value in all, issue slots 74 %
-// busy, 93 us for 8192 rows of 7168).  Here a quotient is a product with the reciprocal and one correction by its exact remainder.  Its
-// error is 2^-23 of a unit in the last place before the rounding, so that it differs from the correctly rounded quotient at most where
-// that lies as close to the middle of two floats; by the constant 448 it is correctly rounded for every significand (all 2^23 compared),
-// so that scales are the same bits, and so are the e4m3 values of bf16 rows (all pairs of significands and 24 exponents compared).
+// busy, 93 us for 8192 rows of 7168).  Here a quotient is a product with the reciprocal and one correction by its exact remainder
+// (Markstein's, of which div_by_shared does two).  Before the last rounding it is off by what the reciprocal and the first product are
+// off by, times what the reciprocal is off by: by __fdividef (2 ulp, 2^-22) 1.25 * 2^-44 of itself, 2^-20 of a unit in the last
+// place or so, by a correctly rounded reciprocal 2^-23.  It differs from the correctly rounded quotient at most where that lies as close to
+// the middle of two floats: by the constant 448 for no significand, so that scales are the same bits, nor are any e4m3 values of bf16
+// rows (tests compare all 2^23, and all pairs of significands 24 exponents apart).  (The norm's fp32 values have no such proof: there
+// an e4m3 value may differ where y / s lies that close to a tie, which the rounding of y moves by more.)
 __device__ __forceinline__ float corrected_quotient(float v, float d, float r) {
   const float q = v * r;
   return fmaf(fmaf(-q, d, v), r, q);
