@@ -587,7 +587,8 @@ const Residents& residents() {
 //   bf16 rows  2.2 for the quantiser's launch, or 0.9 (1.7 where CTAs share SMs) and 0.3 for every group of 128 channels that eight lanes
 //              quantise in the kernel; behind another launch of the same call clusters of 8 take 1.0 longer
 //   CTA pairs  rounds of 0.38 per K block and the epilogue; shared tiles 0.44 and a longer one, as all sums cross shared memory
-// The choice is 1.01 times the best of all kernels and splits on average of 182 such launches, 1.1 times at worst; of 60 of bf16 rows too.
+// The choice takes 1.01 times the best of all kernels and splits on average of 112 products, 1.10 times at worst, 1.00 times of 64 gate/up products,
+// 1.01 (1.05) times of 36 products of bf16 rows; 1 to 2048 tokens.
 struct Choice {
   bool pair;
   int split;
