@@ -244,3 +244,44 @@ def test_weights_written_by_the_kernel_ahead(T, kernel):
         for a, b in zip(outs, want[i % 3]):
             assert torch.isfinite(b).all() and torch.equal(a.view(torch.int16), b.view(torch.int16))
     status()
+
+
+def test_calls_from_several_threads():
+    """Each thread with a stream of its own, all kinds of calls at once: what a call gives alone."""
+    import threading
+
+    K, I, N = 1024, 512, 1032
+    w, ws = weight(N, K, 81)
+    w13, s13 = weight(2 * I, K, 82)
+    w2, s2 = weight(N, I, 83)
+    norm_weight = torch.ones(K, device="cuda")
+    inputs = [rows(T, K, 84 + T, wide=False).bfloat16() for T in (1, 20, 48, 100, 400, 2000)]
+
+    def calls(x):
+        q, s, _ = fg().rms_norm_quant_fp8(x, norm_weight, return_norm=True)
+        y = fg().fp8_block_linear(q, w, ws, x_scale=s)
+        return fg().fp8_gated_mlp(x, w13, s13, w2, s2, addend=y)
+
+    want = [calls(x) for x in inputs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for k in range(60):
+                    j = (i + k) % len(inputs)
+                    got = calls(inputs[j])
+                    if k % 10 == 9 and not torch.equal(got.view(torch.int16), want[j].view(torch.int16)):
+                        wrong.append((i, k))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+    status()
